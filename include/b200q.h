@@ -294,6 +294,33 @@ int b200q_rope_append_paged_gqa_decode(const void* qkv, const float* cos_table, 
                                        int Hkv, int D, int page_size, int64_t num_pages, int max_blocks, int group_size,
                                        float scale, void* stream);
 
+/* Rotary positions on query and key heads, with an optional RMSNorm per head in front: q [T, Hq, D] and k [T, Hkv, D] (k may be
+ * NULL with Hkv = 0) to q_out / k_out, which may be the same memory.  With a weight [D] (in w_dtype) the head is first
+ * y = x * rsqrt(mean(x^2) + eps) * w; then the pairs of its first rotary_dim dimensions - (2i, 2i+1), or with half_layout
+ * (i, i + rotary_dim/2) - are turned by cos / sin [table_len, rotary_dim/2] (fp32) at positions[t]; fp32, rounded once.
+ * (The reference has the interleaved rotation of whole heads only, reference_apply_rope, ops/rope_ops.py:61-75.)
+ *   strides   host array of 8 element strides: token and head of q, of q_out, of k, of k_out; a head is contiguous
+ * A position outside [0, table_len) leaves the head unturned and records event 6.  D up to 1024. */
+int b200q_head_rope(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
+                    const void* k_weight, int w_dtype, float eps, const float* cos_table, const float* sin_table,
+                    const int32_t* positions, int64_t table_len, int rotary_dim, int half_layout, int64_t T, int Hq, int Hkv, int D,
+                    int dtype, void* stream);
+
+/* The same pass over fused rows [q heads | k heads | v heads] (qkv_stride elements apart) that ends in the paged cache: q heads
+ * to q_out [T, Hq, D]; k heads (normalised, turned) and v heads (as they are) to slot positions[t] % page_size of page
+ * block_table[sequences[t], positions[t] / page_size].  sequences NULL: token t belongs to sequence t.  A negative sequence marks
+ * padding: zeros in q_out, nothing else.  No two tokens may share a slot.
+ *   kv_bits   4 or 8: codes and fp16 scales, quantised from the rounded values with the rule of b200q_quantize_kv;
+ *             16: pages [num_pages, page_size, Hkv, D] in the rows' dtype (scales NULL, group_size ignored)
+ * A position outside the table records event 6 (the head is written unturned), a sequence or position without a page event 7
+ * (nothing is appended for it).  b200q_rope_kv_append is the interleaved form for one new token of every sequence. */
+int b200q_norm_rope_kv_append(const void* qkv, int64_t qkv_stride, const float* cos_table, const float* sin_table, int64_t table_len,
+                              int rotary_dim, int half_layout, const int32_t* positions, const int32_t* sequences,
+                              const int32_t* block_table, int B, int max_blocks, const void* q_weight, const void* k_weight, int w_dtype,
+                              float eps, void* q_out, int kv_bits, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                              int64_t T, int Hq, int Hkv, int D, int page_size, int64_t num_pages, int group_size, int dtype,
+                              void* stream);
+
 /* Kernel launches the attention stage takes on the current device for head_dim 128 / page size 16 caches: 1 when the
  * cluster kernel applies (with or without the append), else 2 (split-KV + merge) plus 1 for the append.  For callers
  * that report launch counts; no counterpart in the reference. */

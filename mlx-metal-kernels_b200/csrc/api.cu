@@ -67,6 +67,16 @@ int gemv_read_status(int reset, cudaStream_t stream);
 int attn_read_status(int reset, cudaStream_t stream);
 int peer_read_status(int reset, cudaStream_t stream);
 int stack_read_status(int reset, cudaStream_t stream);
+int rope_read_status(int reset, cudaStream_t stream);
+int head_rope_impl(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
+                   const void* k_weight, int w_dtype, float eps, const float* cos_table, const float* sin_table,
+                   const int32_t* positions, int64_t table_len, int rotary_dim, int half_layout, int64_t T, int Hq, int Hkv, int D,
+                   int dtype, cudaStream_t stream);
+int norm_rope_kv_append_impl(const void* qkv, int64_t qkv_stride, const float* cos_table, const float* sin_table, int64_t table_len,
+                             int rotary_dim, int half_layout, const int32_t* positions, const int32_t* sequences,
+                             const int32_t* block_table, int B, int max_blocks, const void* q_weight, const void* k_weight, int w_dtype,
+                             float eps, void* q_out, int kv_bits, void* k_pages, void* v_pages, void* k_scales, void* v_scales, int64_t T,
+                             int Hq, int Hkv, int D, int page_size, int64_t num_pages, int group_size, int dtype, cudaStream_t stream);
 void scratch_next(void* ptr, size_t bytes);
 size_t scratch_bytes_impl(int rows, int64_t K, int act_dtype);
 size_t norm_scratch_bytes_impl(int rows, int64_t K, int act_dtype);
@@ -383,11 +393,34 @@ int b200q_device_status(int reset, void* stream) {
     const int b = attn_read_status(reset, (cudaStream_t)stream);
     const int c = peer_read_status(reset, (cudaStream_t)stream);
     const int d = stack_read_status(reset, (cudaStream_t)stream);
+    const int e = rope_read_status(reset, (cudaStream_t)stream);
     if (a < 0) return a;
     if (b < 0) return b;
     if (c < 0) return c;
     if (d < 0) return d;
-    return std::max(std::max(a, b), std::max(c, d));
+    if (e < 0) return e;
+    return std::max(std::max(std::max(a, b), std::max(c, d)), e);
+}
+
+int b200q_head_rope(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
+                    const void* k_weight, int w_dtype, float eps, const float* cos_table, const float* sin_table,
+                    const int32_t* positions, int64_t table_len, int rotary_dim, int half_layout, int64_t T, int Hq, int Hkv, int D,
+                    int dtype, void* stream) {
+    tp_discard();
+    return head_rope_impl(q, k, q_out, k_out, strides, q_weight, k_weight, w_dtype, eps, cos_table, sin_table, positions, table_len,
+                          rotary_dim, half_layout, T, Hq, Hkv, D, dtype, (cudaStream_t)stream);
+}
+
+int b200q_norm_rope_kv_append(const void* qkv, int64_t qkv_stride, const float* cos_table, const float* sin_table, int64_t table_len,
+                              int rotary_dim, int half_layout, const int32_t* positions, const int32_t* sequences,
+                              const int32_t* block_table, int B, int max_blocks, const void* q_weight, const void* k_weight, int w_dtype,
+                              float eps, void* q_out, int kv_bits, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                              int64_t T, int Hq, int Hkv, int D, int page_size, int64_t num_pages, int group_size, int dtype,
+                              void* stream) {
+    tp_discard();
+    return norm_rope_kv_append_impl(qkv, qkv_stride, cos_table, sin_table, table_len, rotary_dim, half_layout, positions, sequences,
+                                    block_table, B, max_blocks, q_weight, k_weight, w_dtype, eps, q_out, kv_bits, k_pages, v_pages,
+                                    k_scales, v_scales, T, Hq, Hkv, D, page_size, num_pages, group_size, dtype, (cudaStream_t)stream);
 }
 
 int b200q_peer_allgather(const void* local, void* const* peer_full, uint32_t* const* peer_flags, uint32_t* epoch,

@@ -6,6 +6,7 @@ exception is raised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import os
@@ -42,6 +43,9 @@ SIGNATURES = {
                                   _i, _i64, _i64, _i, _i, _i, _vp]),
     "b200q_rope_append_paged_gqa_decode": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                                 _i, _i, _i, _i, _i, _i64, _i, _i, _f, _vp]),
+    "b200q_head_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _vp, _i64, _i, _i, _i64, _i, _i, _i, _i, _vp]),
+    "b200q_norm_rope_kv_append": (_i, [_vp, _i64, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _f, _vp, _i, _vp, _vp,
+                                       _vp, _vp, _i64, _i, _i, _i, _i, _i64, _i, _i, _vp]),
     "b200q_attention_stage_launches": (_i, [_i, _i, _i]),
     "b200q_attention_launches": (_i, [_i, _i, _i, _i]),
     "b200q_quantize_kv": (_i, [_i, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
@@ -170,6 +174,11 @@ def ptr(t) -> int | None:
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(device):
+    """Context in which the library launches on ``device`` (it launches on the current one)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def contiguous(t):

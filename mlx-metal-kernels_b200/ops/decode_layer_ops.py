@@ -1,5 +1,5 @@
 """Decode-layer glue around the hot-path operators: fused RMSNorm + quantized projection, and
-QKV split + RoPE + quantised KV append.  These are the pieces of the reference's
+QKV split + RoPE + quantised KV append (one new token of every sequence, or any tokens, with head norms).  These are the pieces of the reference's
 llama_layer_decode_step (ops/llama_layer_ops.py:234-428) that sit between the matvec and the
 attention kernels."""
 from __future__ import annotations
@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from . import _cabi
+from .rope_ops import append_launch
 
 
 def norm_quantized_linear(x, norm_weight, w, scales, zeros=None, *, residual_in=None, bits=4, group_size=32, eps=1e-5,
@@ -90,3 +91,33 @@ def rope_append_attention(qkv, cos, sin, positions, paged_qkv, n_heads: int, *, 
         "b200q_rope_append_paged_gqa_decode",
     )
     return out
+
+
+def norm_rope_kv_append(qkv, cos, sin, positions, paged_qkv, n_heads: int, *, sequences=None, q_weight=None, k_weight=None,
+                        eps: float = 1e-6, layout: str = "interleaved"):
+    """``rope_kv_append`` for any tokens: rows qkv [T, (Hq + 2 Hkv) * D] (fp16 / bf16) of the tokens ``positions[t]`` of the
+    sequences ``sequences[t]`` (None: one token of every sequence, in order; negative: padding, whose q row is zeros) ->
+    q [T, Hq, D], turned; the turned k and the v rows go, quantised, into ``paged_qkv`` (a PagedQuantizedKVCache, modified in
+    place; its ``lengths`` are left to the caller).  ``q_weight`` / ``k_weight`` [D]: an RMSNorm of every q / k head in front, in the
+    same pass.  ``cos`` / ``sin`` and ``layout`` as in ``rope_ops.apply_rope``.  No two tokens may share a slot.
+
+    A position outside the table appends the k row unturned and is reported by ``_cabi.device_status()`` (event 6); a token whose
+    sequence or page does not exist appends nothing (event 7).  Nothing is read on the host, so the call can be captured."""
+    shape = paged_qkv.original_page_shape
+    if shape is None:
+        raise ValueError("original_page_shape is required to append")
+    NUM_PAGES, P, Hkv, D = shape
+    bits, group = paged_qkv.bits, paged_qkv.group_size
+    if bits not in (4, 8) or group <= 0:
+        raise ValueError(f"the cache must have 4 or 8 bits and a positive group size, got {bits}, {group}")
+    rows = (NUM_PAGES, P, Hkv)
+    want = {"pages": ((*rows, (D + 1) // 2 if bits == 4 else D), torch.uint8), "scales": ((*rows, -(-D // group)), torch.float16)}
+    for kind, tensors in (("pages", (paged_qkv.k_pages_q, paged_qkv.v_pages_q)), ("scales", (paged_qkv.k_scales, paged_qkv.v_scales))):
+        for t in tensors:
+            if tuple(t.shape) != want[kind][0]:
+                raise ValueError(f"cache {kind} must have shape {want[kind][0]}, got {tuple(t.shape)}")
+            if t.dtype != want[kind][1]:
+                raise TypeError(f"cache {kind} must be {want[kind][1]}, got {t.dtype}")
+    return append_launch(qkv, cos, sin, positions, sequences, paged_qkv.block_table, n_heads, (q_weight, k_weight), eps, layout, bits,
+                         paged_qkv.k_pages_q, paged_qkv.v_pages_q, paged_qkv.k_scales, paged_qkv.v_scales, shape, group,
+                         "norm_rope_kv_append")

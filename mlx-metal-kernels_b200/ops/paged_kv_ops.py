@@ -1,4 +1,4 @@
-"""Block-table gather (reference ops/paged_kv_ops.py:99-182, ops/kv_cache_ops.py:37-61) and decode attention over
+"""Block-table gather (reference ops/paged_kv_ops.py:99-182, ops/kv_cache_ops.py:37-61), append to and decode attention over
 an unquantised paged cache (ops/paged_kv_ops.py:258-360, ops/gqa_ops.py:307-340)."""
 from __future__ import annotations
 
@@ -7,6 +7,7 @@ import math
 import torch
 
 from . import _cabi
+from .rope_ops import append_launch
 
 
 def make_identity_block_table(B: int, MAX_S: int, PAGE_SIZE: int, device=None) -> torch.Tensor:
@@ -155,3 +156,15 @@ def paged_decode_attention(q, K_pages, V_pages, block_table, lengths, *, scale=N
         raise TypeError(f"q dtype must be float16 or bfloat16, got {q.dtype}")
     _cabi.require_cuda(q, K_pages, V_pages, block_table, lengths_arr)
     return paged_fp16_attention_launch(q.reshape(B, H, D), K_pages, V_pages, block_table, lengths_arr, scale).reshape(B, 1, H, D)
+
+
+def norm_rope_kv_append_pages(qkv, cos, sin, positions, K_pages, V_pages, block_table, n_heads: int, *, sequences=None, q_weight=None,
+                              k_weight=None, eps: float = 1e-6, layout: str = "interleaved"):
+    """``decode_layer_ops.norm_rope_kv_append`` for plain pages [NUM_PAGES,PAGE_SIZE,Hkv,D] in the dtype of the rows (modified in
+    place): q [T, n_heads, D] turned, k (turned) and v written to the slots of their tokens as they are.  The reference's update
+    kernels copy the whole cache per token (kernels/paged_kv_cache_update.metal)."""
+    NUM_PAGES, PAGE_SIZE, Hkv, D, _, _ = _validate_page_tensors(K_pages, V_pages, block_table)
+    if K_pages.dtype != qkv.dtype or V_pages.dtype != qkv.dtype:
+        raise TypeError(f"pages must have the dtype of the rows, got {K_pages.dtype}, {V_pages.dtype} and {qkv.dtype}")
+    return append_launch(qkv, cos, sin, positions, sequences, block_table, n_heads, (q_weight, k_weight), eps, layout, 16, K_pages, V_pages,
+                         None, None, (NUM_PAGES, PAGE_SIZE, Hkv, D), 0, "norm_rope_kv_append_pages")
