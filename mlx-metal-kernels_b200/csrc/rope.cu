@@ -11,6 +11,9 @@
 // (normalised, rotated) and the v heads (as they are) to slot pos % P of page block_table[sequence, pos / P]: as they are, or
 // quantised from the rounded values with the cache's rule (see stack.cu).
 //
+// Bound by HBM for prompts and by latency for a few tokens.  A head is taken by D/16 lanes, so that a lane has two 16-byte pieces
+// of it: pieces l and l + D/16, which are the two halves of eight pairs in the half layout over whole heads.  Four
+// heads of one token per lane keep eight loads in flight and share the token's cos / sin and the norm's weights.
 #include "common.cuh"
 
 #include <algorithm>
@@ -21,7 +24,11 @@ B200Q_DEFINE_STATUS_WORD(rope_read_status)
 
 namespace {
 
+constexpr int kRun = 4;          // heads of one token and kind that a group of lanes takes
+constexpr int kThreads = 256;
+
 enum HeadKind : int { KIND_Q = 0, KIND_K = 1, KIND_V = 2 };
+enum Layout : int { INTERLEAVED = 0, HALF_WHOLE = 1, HALF_PART = 2 };
 enum CacheKind : int { NO_CACHE = 0, CACHE_Q4 = 4, CACHE_Q8 = 8, CACHE_PLAIN = 16 };
 
 struct RopeParams {
@@ -37,10 +44,48 @@ struct RopeParams {
     void* codes[3];               // k and v pages at KIND_K, KIND_V
     __half* scales[3];
     int64_t T, table_len, num_pages;
-    int heads[3];                 // heads per kind
+    int heads[3], runs[3];        // heads per kind, and groups of kRun of them
     int B, max_blocks, P, D, R, G, w_dtype;
     float eps;
 };
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8], const __half*) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8], const __nv_bfloat16*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    return *reinterpret_cast<const uint4*>(e);
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load_weight8(const void* w, int dtype, int i, float (&v)[8]) {
+    if (dtype == B200Q_F32) {
+        load8(reinterpret_cast<const float*>(w) + i, v);
+    } else {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(w) + i));
+        if (dtype == B200Q_F16) unpack8(u, v, (const __half*)nullptr);
+        else unpack8(u, v, (const __nv_bfloat16*)nullptr);
+    }
+}
 
 // (u, v) turned: separately rounded products and one sum, as elementwise operations give it
 __device__ __forceinline__ float turn_u(float u, float v, float c, float s) { return __fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s)); }
@@ -64,7 +109,193 @@ template <int CACHE> __device__ __forceinline__ uint32_t kv_code(float v, float 
     return (uint32_t)(int)(fminf(fmaxf(rintf(__fdiv_rn(v, scale)), -limit), limit) + offset);
 }
 
-// Any head size, rotary size, group size, stride and alignment: one warp per (token, head), the head in shared memory.
+// D a power of two from 32 to 256, R a multiple of 16, groups of whole pieces, everything aligned to 16 bytes.
+template <typename T, int LAYOUT, int CACHE>
+__global__ void __launch_bounds__(kThreads) rope_heads_kernel(const __grid_constant__ RopeParams p, int log_lanes, int64_t units) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lanes = 1 << log_lanes;                        // lanes of a head: D / 16
+    const int l = threadIdx.x & (lanes - 1);
+    const int64_t unit = (int64_t)blockIdx.x * (kThreads >> log_lanes) + (threadIdx.x >> log_lanes);
+    const bool live = unit < units;
+    const int per_token = p.runs[0] + p.runs[1] + p.runs[2];
+    const int64_t t = live ? unit / per_token : 0;
+    int run = live ? (int)(unit - t * per_token) : 0;
+    int kind = KIND_Q;
+    if (run >= p.runs[0]) { run -= p.runs[0]; kind = KIND_K; }
+    if (kind == KIND_K && run >= p.runs[1]) { run -= p.runs[1]; kind = KIND_V; }
+    const int h0 = run * kRun;
+    const int count = live ? min(kRun, p.heads[kind] - h0) : 0;
+    const int d0 = l * 8, d1 = (l + lanes) * 8;              // first dimension of the lane's two pieces
+
+    const T* src = reinterpret_cast<const T*>(p.in[kind]) + t * p.in_token[kind] + (int64_t)h0 * p.in_head[kind];
+    uint4 x0[kRun], x1[kRun], o0[kRun], o1[kRun];            // o: the partners of the pieces, where another lane owns them
+    const int half = p.R / 2;
+    const bool turns = kind != KIND_V;
+    const int partner0 = d0 < half ? d0 + half : d0 - half, partner1 = d1 < half ? d1 + half : d1 - half;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+        x0[j] = x1[j] = o0[j] = o1[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (j < count) {
+            const T* row = src + j * p.in_head[kind];
+            x0[j] = *reinterpret_cast<const uint4*>(row + d0);
+            x1[j] = *reinterpret_cast<const uint4*>(row + d1);
+            if (LAYOUT == HALF_PART && turns) {
+                if (d0 < p.R) o0[j] = *reinterpret_cast<const uint4*>(row + partner0);
+                if (d1 < p.R) o1[j] = *reinterpret_cast<const uint4*>(row + partner1);
+            }
+        }
+    }
+    const int pos = live ? p.positions[t] : 0;
+    const int seq = CACHE != NO_CACHE && live ? (p.sequences ? p.sequences[t] : (int)t) : 0;
+    const bool padding = CACHE != NO_CACHE && seq < 0;
+    const bool in_table = pos >= 0 && pos < p.table_len;
+    const bool rotate = turns && in_table && !padding && live;
+    if (live && turns && !in_table && !padding && l == 0) atomicMax(&g_device_status, (int)EV_ROPE_POSITION);
+
+    // cos / sin: LAYOUT INTERLEAVED: four pairs of each piece; HALF_WHOLE: eight pairs; HALF_PART: eight pairs of each piece
+    float c0[8], s0[8], c1[8], s1[8];
+    if (rotate) {
+        const float* ct = p.cos_table + (int64_t)pos * half;
+        const float* st = p.sin_table + (int64_t)pos * half;
+        if (LAYOUT == HALF_WHOLE) {
+            load8(ct + d0, c0);
+            load8(st + d0, s0);
+        } else if (LAYOUT == HALF_PART) {
+            if (d0 < p.R) { load8(ct + min(d0, partner0), c0); load8(st + min(d0, partner0), s0); }
+            if (d1 < p.R) { load8(ct + min(d1, partner1), c1); load8(st + min(d1, partner1), s1); }
+        } else {
+            auto load4 = [](const float* q, float (&v)[8]) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(q));
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            };
+            if (d0 < p.R) { load4(ct + d0 / 2, c0); load4(st + d0 / 2, s0); }
+            if (d1 < p.R) { load4(ct + d1 / 2, c1); load4(st + d1 / 2, s1); }
+        }
+    }
+    const void* weight = p.weight[kind];
+    float w0[8], w1[8], wo0[8], wo1[8];
+    if (weight != nullptr && live) {
+        load_weight8(weight, p.w_dtype, d0, w0);
+        load_weight8(weight, p.w_dtype, d1, w1);
+        if (LAYOUT == HALF_PART) {
+            if (d0 < p.R) load_weight8(weight, p.w_dtype, partner0, wo0);
+            if (d1 < p.R) load_weight8(weight, p.w_dtype, partner1, wo1);
+        }
+    }
+    int64_t row_index = -1;                                  // slot in the pool, in tokens
+    if (CACHE != NO_CACHE && live && kind != KIND_Q) row_index = cache_row(p, t, pos, seq, l == 0);
+    if (LAYOUT == HALF_PART) __syncwarp();                   // in place: nobody stores before the partners are loaded
+
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+        float a[8], b[8];
+        unpack8(x0[j], a, (const T*)nullptr);
+        unpack8(x1[j], b, (const T*)nullptr);
+        float inv = 1.0f;
+        if (weight != nullptr) {                             // uniform over the lanes of a head
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+            const unsigned group = (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (threadIdx.x & 31 & ~(lanes - 1));
+            for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(group, ss, o);
+            inv = rsqrtf(ss / (float)p.D + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] = a[i] * inv * w0[i];
+                b[i] = b[i] * inv * w1[i];
+            }
+        }
+        if (rotate) {
+            if (LAYOUT == HALF_WHOLE) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float u = a[i], v = b[i];
+                    a[i] = turn_u(u, v, c0[i], s0[i]);
+                    b[i] = turn_v(u, v, c0[i], s0[i]);
+                }
+            } else if (LAYOUT == HALF_PART) {
+                auto half_part = [&](float (&x)[8], const uint4& other, const float (&wo)[8], const float (&c)[8], const float (&s)[8], bool low) {
+                    float y[8];
+                    unpack8(other, y, (const T*)nullptr);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (weight != nullptr) y[i] = y[i] * inv * wo[i];
+                        x[i] = low ? turn_u(x[i], y[i], c[i], s[i]) : turn_v(y[i], x[i], c[i], s[i]);
+                    }
+                };
+                if (d0 < p.R) half_part(a, o0[j], wo0, c0, s0, d0 < half);
+                if (d1 < p.R) half_part(b, o1[j], wo1, c1, s1, d1 < half);
+            } else {
+                auto pairs = [](float (&x)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float u = x[2 * i], v = x[2 * i + 1];
+                        x[2 * i] = turn_u(u, v, c[i], s[i]);
+                        x[2 * i + 1] = turn_v(u, v, c[i], s[i]);
+                    }
+                };
+                if (d0 < p.R) pairs(a, c0, s0);
+                if (d1 < p.R) pairs(b, c1, s1);
+            }
+        }
+        const uint4 y0 = pack8<T>(a), y1 = pack8<T>(b);
+        if (CACHE == NO_CACHE || kind == KIND_Q) {
+            if (j < count) {
+                T* row = reinterpret_cast<T*>(p.out[kind]) + t * p.out_token[kind] + (int64_t)(h0 + j) * p.out_head[kind];
+                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(row + d0) = padding ? zero : y0;
+                *reinterpret_cast<uint4*>(row + d1) = padding ? zero : y1;
+            }
+        } else if (CACHE == CACHE_PLAIN) {
+            if (j < count && row_index >= 0) {
+                T* row = reinterpret_cast<T*>(p.codes[kind]) + (row_index * p.heads[kind] + h0 + j) * p.D;
+                *reinterpret_cast<uint4*>(row + d0) = y0;
+                *reinterpret_cast<uint4*>(row + d1) = y1;
+            }
+        } else {
+            // the values as the cache sees them: rounded to T.  Group maxima over the G/8 neighbouring lanes; a group of the
+            // whole head takes both pieces of every lane
+            unpack8(y0, a, (const T*)nullptr);
+            unpack8(y1, b, (const T*)nullptr);
+            float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                m0 = fmaxf(m0, fabsf(a[i]));
+                m1 = fmaxf(m1, fabsf(b[i]));
+            }
+            const int pieces = p.G / 8;
+            if (pieces > lanes) m0 = m1 = fmaxf(m0, m1);
+            const unsigned group = (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (threadIdx.x & 31 & ~(lanes - 1));
+            for (int o = 1; o < min(pieces, lanes); o <<= 1) {
+                m0 = fmaxf(m0, __shfl_xor_sync(group, m0, o));
+                m1 = fmaxf(m1, __shfl_xor_sync(group, m1, o));
+            }
+            if (j < count && row_index >= 0) {
+                constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f;
+                const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
+                const int64_t row = row_index * p.heads[kind] + h0 + j;
+                auto store = [&](const float (&v)[8], float scale, int d) {
+                    uint32_t c[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
+                    uint8_t* codes = reinterpret_cast<uint8_t*>(p.codes[kind]);
+                    if (CACHE == CACHE_Q8)
+                        *reinterpret_cast<uint2*>(codes + row * p.D + d) =
+                            make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+                    else
+                        *reinterpret_cast<uint32_t*>(codes + (row * p.D + d) / 2) =
+                            c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12 | c[4] << 16 | c[5] << 20 | c[6] << 24 | c[7] << 28;
+                    if (d % p.G == 0) p.scales[kind][row * (p.D / p.G) + d / p.G] = __float2half_rn(scale);
+                };
+                store(a, q0, d0);
+                store(b, q1, d1);
+            }
+        }
+    }
+}
+
+// Every other head size, rotary size, group size, stride and alignment: one warp per (token, head), the head in shared memory.
 constexpr int kAnyWarps = 4, kAnyMaxDim = 1024;
 template <typename T, int CACHE>
 __global__ void __launch_bounds__(kAnyWarps * 32) rope_any_kernel(const __grid_constant__ RopeParams p, bool half_layout, int64_t units) {
@@ -140,6 +371,15 @@ __global__ void __launch_bounds__(kAnyWarps * 32) rope_any_kernel(const __grid_c
     }
 }
 
+bool aligned16(const RopeParams& p) {
+    uintptr_t bits = (uintptr_t)p.cos_table | (uintptr_t)p.sin_table;
+    for (int i = 0; i < 3; ++i) {
+        bits |= (uintptr_t)p.in[i] | (uintptr_t)p.out[i] | (uintptr_t)p.weight[i] | (uintptr_t)p.codes[i];
+        bits |= (uintptr_t)((p.in_token[i] | p.in_head[i] | p.out_token[i] | p.out_head[i]) * 2);
+    }
+    return (bits & 15u) == 0;
+}
+
 template <typename K, typename... A>
 int launch(K kernel, int64_t blocks, int threads, size_t smem, cudaStream_t stream, A... args) {
     if (blocks > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
@@ -159,6 +399,18 @@ int launch(K kernel, int64_t blocks, int threads, size_t smem, cudaStream_t stre
 
 template <typename T, int CACHE>
 int dispatch(RopeParams& p, bool half_layout, cudaStream_t stream) {
+    const bool pow2 = (p.D & (p.D - 1)) == 0 && p.D >= 32 && p.D <= 256;
+    const bool groups = (CACHE != CACHE_Q4 && CACHE != CACHE_Q8) || (p.G % 8 == 0 && (p.G & (p.G - 1)) == 0 && p.D % p.G == 0);
+    if (pow2 && p.R % 16 == 0 && groups && aligned16(p)) {
+        int log_lanes = 1;
+        while ((16 << log_lanes) < p.D) ++log_lanes;
+        for (int i = 0; i < 3; ++i) p.runs[i] = (p.heads[i] + kRun - 1) / kRun;
+        const int64_t units = p.T * (p.runs[0] + p.runs[1] + p.runs[2]), per_block = kThreads >> log_lanes;
+        const int64_t blocks = (units + per_block - 1) / per_block;
+        if (!half_layout) return launch(rope_heads_kernel<T, INTERLEAVED, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
+        if (p.R == p.D) return launch(rope_heads_kernel<T, HALF_WHOLE, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
+        return launch(rope_heads_kernel<T, HALF_PART, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
+    }
     const int64_t units = p.T * (p.heads[0] + p.heads[1] + p.heads[2]);
     return launch(rope_any_kernel<T, CACHE>, (units + kAnyWarps - 1) / kAnyWarps, kAnyWarps * 32, sizeof(float) * kAnyWarps * p.D, stream, p,
                   half_layout, units);
