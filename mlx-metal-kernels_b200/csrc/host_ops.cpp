@@ -50,6 +50,12 @@ int (*p_plain_checked)(const void*, const void*, const void*, const int32_t*, co
 int (*p_quant_pair)(int, const void*, const void*, uint8_t*, uint8_t*, void*, void*, int64_t, int, int, int, void*) = nullptr;
 int (*p_dequant_pair)(int, const uint8_t*, const uint8_t*, const void*, const void*, void*, void*, int64_t, int, int, void*) = nullptr;
 
+int (*p_head_rope)(const void*, const void*, void*, void*, const int64_t*, const void*, const void*, int, float, const float*, const float*,
+                   const int32_t*, int64_t, int, int, int64_t, int, int, int, int, void*) = nullptr;
+int (*p_append)(const void*, int64_t, const float*, const float*, int64_t, int, int, const int32_t*, const int32_t*, const int32_t*, int, int,
+                const void*, const void*, int, float, void*, int, void*, void*, void*, void*, int64_t, int, int, int, int, int64_t, int, int,
+                void*) = nullptr;
+
 constexpr int kMaxDevices = 64;
 constexpr int kErrUnsupported = -2, kErrWorkspace = -4;      // B200Q_ERR_*
 constexpr int kMinNormRows = 5;      // from this many rows on the library runs the rmsnorm as a launch of its own
@@ -90,6 +96,8 @@ bool matrix(Matrix& m, PyObject* w, PyObject* s, PyObject* z, int bits, int64_t 
 }
 const void* ptr(const Tensor* t) { return t == nullptr ? nullptr : t->const_data_ptr(); }
 const uint8_t* codes(const Tensor* t) { return static_cast<const uint8_t*>(t->const_data_ptr()); }
+
+const int32_t* i32(const Tensor* t) { return static_cast<const int32_t*>(ptr(t)); }
 
 Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, int dev) {
     return at::detail::empty_cuda(shape, dtype, at::Device(at::kCUDA, dev), std::nullopt);
@@ -235,7 +243,6 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         ws_bytes = p_attn_ws((int)B, (int)Hq, (int)Hkv, (int)D);
         ws = empty({(int64_t)ws_bytes}, at::kByte, dev);
     }
-    const auto i32 = [](const Tensor* t) { return static_cast<const int32_t*>(t->const_data_ptr()); };
     void* wp = ws_bytes ? ws.mutable_data_ptr() : nullptr;
     const int act = dtype_code(q->scalar_type()), sdt = dtype_code(ks->scalar_type()), mb = (int)bt->size(1);
     const int rc = window > 0
@@ -402,6 +409,120 @@ PyObject* dequantize_kv(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return rc == 0 ? tuple_of({&k, &v}) : none();
 }
 
+// What the rotation operators share: tables, positions, norm weights and layout on one device.
+struct Rotation {
+    const Tensor *cos, *sin, *pos, *qw, *kw;
+    int w_dtype = 2, half = 0;
+    float eps = 0.0f;
+};
+bool rotation(Rotation& r, PyObject* cos, PyObject* sin, PyObject* pos, PyObject* qw, PyObject* kw, PyObject* eps, PyObject* layout, int64_t D,
+              int dev) {
+    r.cos = as_tensor(cos);
+    r.sin = as_tensor(sin);
+    r.pos = as_tensor(pos);
+    r.qw = as_tensor(qw);
+    r.kw = as_tensor(kw);
+    if (!r.cos || !r.sin || !r.pos || (!r.qw && qw != Py_None) || (!r.kw && kw != Py_None) || !PyFloat_Check(eps)) return false;
+    r.eps = (float)PyFloat_AS_DOUBLE(eps);
+    r.half = one_of(layout, {"half"}) ? 1 : 0;
+    if (!(r.eps >= 0.0f) || (!r.half && !one_of(layout, {"interleaved"}))) return false;
+    if (!on(*r.cos, dev) || !on(*r.sin, dev) || !on(*r.pos, dev) || r.cos->dim() != 2 || r.cos->sizes() != r.sin->sizes() ||
+        r.cos->scalar_type() != at::kFloat || r.sin->scalar_type() != at::kFloat || r.pos->scalar_type() != at::kInt)
+        return false;
+    if (r.cos->size(0) <= 0 || r.cos->size(1) <= 0 || 2 * r.cos->size(1) > D || D > 1024) return false;
+    for (const Tensor* w : {r.qw, r.kw}) {
+        if (w == nullptr) continue;
+        if (!on(*w, dev) || w->dim() != 1 || w->size(0) != D || dtype_code(w->scalar_type()) < 0) return false;
+        r.w_dtype = dtype_code(w->scalar_type());
+    }
+    return r.qw == nullptr || r.kw == nullptr || r.qw->scalar_type() == r.kw->scalar_type();
+}
+const float* f32(const Tensor* t) { return static_cast<const float*>(t->const_data_ptr()); }
+
+// stride of the tokens of x [..., H, D] with contiguous heads when the leading dimensions (one or two) have one; else false
+bool token_stride(const Tensor& x, int64_t* stride) {
+    const int64_t n = x.dim();
+    if (x.stride(n - 1) != 1 && x.size(n - 1) != 1) return false;
+    if (n == 4 && x.size(0) != 1 && x.stride(0) != x.size(1) * x.stride(1)) return false;
+    *stride = x.stride(n - 3);
+    return true;
+}
+
+// head_rope(q, k or None, q_weight or None, k_weight or None, cos, sin, positions, eps, layout) -> (q, k or None) or None
+PyObject* head_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (p_head_rope == nullptr || n_args != 9) return none();
+    const Tensor *q = as_tensor(a[0]), *k = as_tensor(a[1]);
+    const int dev = current_device_of(q);
+    if (dev < 0 || (k == nullptr && a[1] != Py_None) || (q->dim() != 3 && q->dim() != 4) || !act_dtype(q->scalar_type())) return none();
+    const int64_t n = q->dim(), Hq = q->size(n - 2), D = q->size(n - 1), Hkv = k == nullptr ? 0 : k->size(n - 2);
+    int64_t T = 1, qs = 0, ks = 0;
+    for (int64_t i = 0; i < n - 2; ++i) T *= q->size(i);
+    Rotation r;
+    if (T <= 0 || Hq <= 0 || D <= 0 || Hq > INT32_MAX || Hkv > INT32_MAX || !token_stride(*q, &qs) ||
+        !rotation(r, a[4], a[5], a[6], a[2], a[3], a[7], a[8], D, dev))
+        return none();
+    if (r.pos->sizes() != q->sizes().slice(0, n - 2)) return none();
+    if (k != nullptr && (!k->is_cuda() || k->get_device() != dev || k->dim() != n || k->scalar_type() != q->scalar_type() || Hkv <= 0 ||
+                         k->size(n - 1) != D || k->sizes().slice(0, n - 2) != q->sizes().slice(0, n - 2) || !token_stride(*k, &ks)))
+        return none();
+    Tensor qo = empty(q->sizes(), q->scalar_type(), dev), ko;
+    if (k != nullptr) ko = empty(k->sizes(), k->scalar_type(), dev);
+    const int64_t strides[8] = {qs, q->stride(n - 2), Hq * D, D, ks, k == nullptr ? 0 : k->stride(n - 2), Hkv * D, D};
+    const int rc = p_head_rope(q->const_data_ptr(), ptr(k), qo.mutable_data_ptr(), k == nullptr ? nullptr : ko.mutable_data_ptr(), strides,
+                               ptr(r.qw), ptr(r.kw), r.w_dtype, r.eps, f32(r.cos), f32(r.sin), i32(r.pos), r.cos->size(0),
+                               (int)(2 * r.cos->size(1)), r.half, T, (int)Hq, (int)Hkv, (int)D, dtype_code(q->scalar_type()), stream_of(dev));
+    if (rc != 0) return none();
+    PyObject* out = PyTuple_New(2);
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
+    if (k == nullptr) Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(out, 1, k == nullptr ? Py_None : THPVariable_Wrap(std::move(ko)));
+    return out;
+}
+
+// norm_rope_append(qkv, cos, sin, positions, sequences or None, block_table, n_heads, q_weight, k_weight, eps, layout, bits, k pages, v pages,
+//                  k scales or None, v scales or None, group_size, shape) -> q or None
+PyObject* norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    int64_t Hq, bits, group, dims[4];
+    if (p_append == nullptr || n_args != 18 || !as_int(a[6], &Hq) || !as_int(a[11], &bits) || !as_int(a[16], &group) || !PyTuple_Check(a[17]) ||
+        PyTuple_GET_SIZE(a[17]) != 4)
+        return none();
+    for (int i = 0; i < 4; ++i)
+        if (!as_int(PyTuple_GET_ITEM(a[17], i), &dims[i]) || dims[i] <= 0) return none();
+    const int64_t pages = dims[0], P = dims[1], Hkv = dims[2], D = dims[3];
+    const Tensor *x = as_tensor(a[0]), *seq = as_tensor(a[4]), *bt = as_tensor(a[5]);
+    const int dev = current_device_of(x);
+    if (dev < 0 || bt == nullptr || (seq == nullptr && a[4] != Py_None) || x->dim() != 2 || !act_dtype(x->scalar_type()) || Hq <= 0 ||
+        Hq > INT32_MAX || Hkv > INT32_MAX || P > INT32_MAX || x->size(0) <= 0 || x->size(1) != (Hq + 2 * Hkv) * D || x->stride(1) != 1 ||
+        x->stride(0) < x->size(1))
+        return none();
+    const int64_t T = x->size(0);
+    Rotation r;
+    if (!rotation(r, a[1], a[2], a[3], a[7], a[8], a[9], a[10], D, dev) || r.pos->dim() != 1 || r.pos->size(0) != T) return none();
+    if (!on(*bt, dev) || bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) <= 0 || bt->size(1) <= 0 || bt->size(0) > INT32_MAX ||
+        bt->size(1) > INT32_MAX)
+        return none();
+    if (seq == nullptr ? T != bt->size(0) : !on(*seq, dev) || seq->scalar_type() != at::kInt || seq->dim() != 1 || seq->size(0) != T) return none();
+    const bool plain = bits == 16;
+    if (!plain && ((bits != 4 && bits != 8) || group <= 0 || group > INT32_MAX)) return none();
+    const Tensor *kp = as_tensor(a[12]), *vp = as_tensor(a[13]), *ks = as_tensor(a[14]), *vs = as_tensor(a[15]);
+    const int64_t slots = pages * P * Hkv, width = bits == 4 ? (D + 1) / 2 : D;
+    for (const Tensor* t : {kp, vp})
+        if (t == nullptr || !on(*t, dev) || t->scalar_type() != (plain ? x->scalar_type() : at::kByte) || t->dim() != 4 || t->size(0) != pages ||
+            t->size(1) != P || t->size(2) != Hkv || t->size(3) != width)
+            return none();
+    for (const Tensor* t : {ks, vs})
+        if (!plain && (t == nullptr || !on(*t, dev) || t->scalar_type() != at::kHalf || t->dim() != 4 || t->size(0) != pages || t->size(1) != P ||
+                       t->size(2) != Hkv || t->numel() != slots * ((D + group - 1) / group)))
+            return none();
+    Tensor out = empty({T, Hq, D}, x->scalar_type(), dev);
+    const auto w = [](const Tensor* t) { return t == nullptr ? nullptr : t->mutable_data_ptr(); };
+    const int rc = p_append(x->const_data_ptr(), x->stride(0), f32(r.cos), f32(r.sin), r.cos->size(0), (int)(2 * r.cos->size(1)), r.half,
+                            i32(r.pos), i32(seq), i32(bt), (int)bt->size(0), (int)bt->size(1), ptr(r.qw), ptr(r.kw), r.w_dtype, r.eps,
+                            out.mutable_data_ptr(), (int)bits, w(kp), w(vp), plain ? nullptr : w(ks), plain ? nullptr : w(vs), T, (int)Hq,
+                            (int)Hkv, (int)D, (int)P, pages, plain ? 0 : (int)group, dtype_code(x->scalar_type()), stream_of(dev));
+    return rc == 0 ? THPVariable_Wrap(std::move(out)) : none();
+}
+
 // bind({symbol: address}): the C ABI functions to call
 PyObject* bind(PyObject*, PyObject* table) {
     const struct { const char* name; void** slot; } want[] = {
@@ -411,6 +532,7 @@ PyObject* bind(PyObject*, PyObject* table) {
         {"b200q_paged_gqa_decode", (void**)&p_attn}, {"b200q_paged_gqa_decode_window", (void**)&p_attn_window},
         {"b200q_paged_fp16_gqa_workspace_bytes", (void**)&p_plain_ws}, {"b200q_paged_fp16_gqa_decode", (void**)&p_plain_attn},
         {"b200q_paged_fp16_gqa_decode_checked", (void**)&p_plain_checked},
+        {"b200q_head_rope", (void**)&p_head_rope}, {"b200q_norm_rope_kv_append", (void**)&p_append},
         {"b200q_quantize_kv_pair", (void**)&p_quant_pair}, {"b200q_dequantize_kv_pair", (void**)&p_dequant_pair},
     };
     for (const auto& w : want) {
@@ -440,6 +562,8 @@ PyMethodDef methods[] = {
     {"mlp_block", FAST(mlp_block), METH_FASTCALL, nullptr},
     {"quantize_kv", FAST(quantize_kv), METH_FASTCALL, nullptr},
     {"dequantize_kv", FAST(dequantize_kv), METH_FASTCALL, nullptr},
+    {"head_rope", FAST(head_rope), METH_FASTCALL, nullptr},
+    {"norm_rope_append", FAST(norm_rope_append), METH_FASTCALL, nullptr},
     {"plain_attention", FAST(plain_attention), METH_FASTCALL, nullptr},
     {"paged_attention", FAST(paged_attention), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -247,6 +247,10 @@ def apply_rope(q, k, cos, sin, positions, *, layout: str = "interleaved", inplac
 
     q and k may be strided views (slices of the fused rows).  A position outside the table leaves its heads unturned and is
     reported by ``_cabi.device_status()`` (event 6); nothing is read on the host, so the call can be captured."""
+    if not inplace:
+        out = _cabi.host().head_rope(q, k, None, None, cos, sin, positions, 0.0, layout)
+        if out is not None:
+            return out
     return _head_rope(q, k, (None, None), cos, sin, positions, 0.0, layout, inplace, "apply_rope")
 
 
@@ -254,7 +258,11 @@ def head_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float 
                    inplace: bool = False):
     """``apply_rope`` with an RMSNorm of every head in front, in the same pass: y = x * rsqrt(mean(x^2) + eps) * weight over the
     whole head, not rounded before the rotation.  A weight [D] of None leaves its heads as they are."""
-    if eps < 0:
+    if not inplace:
+        out = _cabi.host().head_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, layout)
+        if out is not None:
+            return out
+    if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     return _head_rope(q, k, (q_weight, k_weight), cos, sin, positions, eps, layout, inplace, "head_norm_rope")
 
@@ -262,6 +270,10 @@ def head_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float 
 def append_launch(qkv, cos, sin, positions, sequences, block_table, n_heads, weights, eps, layout, kv_bits, k_pages, v_pages, k_scales,
                   v_scales, page_shape, group_size, who):
     """Checks and launch of the append form for both kinds of pages; ``page_shape`` (NUM_PAGES, PAGE_SIZE, Hkv, D)."""
+    out = _cabi.host().norm_rope_append(qkv, cos, sin, positions, sequences, block_table, n_heads, *weights, eps, layout, kv_bits, k_pages,
+                                        v_pages, k_scales, v_scales, group_size, page_shape)
+    if out is not None:
+        return out
     num_pages, page_size, Hkv, D = page_shape
     if qkv.ndim != 2 or qkv.shape[1] != (n_heads + 2 * Hkv) * D or n_heads <= 0:
         raise ValueError(f"qkv must be [T, (n_heads + 2 * {Hkv}) * {D}] with n_heads = {n_heads}, got {tuple(qkv.shape)}")
@@ -280,7 +292,7 @@ def append_launch(qkv, cos, sin, positions, sequences, block_table, n_heads, wei
         raise ValueError(f"sequences must have shape {(T,)}, got {tuple(sequences.shape)}")
     if not 0 < D <= _MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be in [1, {_MAX_HEAD_DIM}], got {D}")
-    if eps < 0:
+    if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     half = layout_code(layout)
     cos, sin = check_tables(cos, sin, D)
