@@ -49,7 +49,8 @@ const char* b200q_strerror(int code);
 /* Reads (and, if reset != 0, clears) the device-side status word.  Kernels record an event there instead of
  * trapping: 1-5 a bounded wait (on a shared-memory barrier or on a peer's flag) ran out, 6 b200q_rope_kv_append
  * met a position outside the rotary table (the row was left unrotated), 7 it met a position whose block-table
- * entry is unassigned (nothing was appended).  The largest event seen is returned.  Synchronises `stream`.
+ * entry is unassigned (nothing was appended), 8 a page operator met indices, lengths or counts that it cannot take, 9 it
+ * found too few free pages.  The largest event seen is returned.  Synchronises `stream`.
  * 0 = no event. */
 int b200q_device_status(int reset, void* stream);
 
@@ -345,6 +346,41 @@ int b200q_quantize_kv_pair(int bits, const void* k, const void* v, uint8_t* k_co
                            void* v_scales, int64_t rows, int D, int group_size, int in_dtype, void* stream);
 int b200q_dequantize_kv_pair(int bits, const uint8_t* k_codes, const uint8_t* v_codes, const void* k_scales,
                              const void* v_scales, void* k, void* v, int64_t rows, int D, int group_size, void* stream);
+
+/* Pages of the paged caches of all layers (no counterpart in the reference, whose block tables are static): one block table
+ * [B, max_blocks] (entries < 0: unassigned), one length per sequence and one array of reference counts [num_pages] (int32; 0: free)
+ * for all layers, whose tensors are given as two groups of HOST arrays of device pointers: bases0[n0] with slot0 bytes per token
+ * slot of a page (codes, or plain values), bases1[n1] with slot1 (scales; n1 = 0 for plain pages); page p of a tensor is its
+ * page_size * slot bytes from p * page_size * slot on.  Everything happens on the device, in stream order, without a word to the host; calls on
+ * one set of counts must be stream-ordered.  The lowest free pages are taken, in the order of the call.  Indices below 0 are padding.
+ * A call that cannot be served changes nothing and records event 8 (indices, lengths) or 9 (too few free pages); the release
+ * records event 8 for what it skips.  Workspaces: device scratch of the matching *_workspace_bytes, 16-byte aligned. */
+size_t b200q_reserve_pages_workspace_bytes(int B, int64_t num_pages);
+size_t b200q_copy_pages_workspace_bytes(int n, int64_t num_pages);
+size_t b200q_fork_sequences_workspace_bytes(int n, int B);
+size_t b200q_compact_pages_workspace_bytes(int64_t num_pages);
+/* Every sequence b gets a page of its own for each unassigned block of the positions lengths[b] ... lengths[b] + new - 1, new =
+ * new_tokens[b] or, with new_tokens NULL, `uniform`; rows in order, blocks in order. */
+int b200q_reserve_pages(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, const int32_t* lengths, const int32_t* new_tokens,
+                        int uniform, int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes, void* stream);
+/* The sequences rows[n] give up their pages: counts fall by one per entry, entries become -1, lengths 0.  A row listed twice is
+ * released once.  A row >= B is skipped, an entry whose page nobody held leaves its count alone; both record event 8. */
+int b200q_release_sequences(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* rows, int n,
+                            int B, int max_blocks, void* stream);
+/* Page src[i] to page dst[i] in every tensor, i < n.  The destinations must differ from one another and from every source. */
+int b200q_copy_pages(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, const int32_t* src,
+                     const int32_t* dst, int n, int64_t num_pages, int page_size, void* workspace, size_t workspace_bytes, void* stream);
+/* Sequence children[i] continues as parents[i] does now: it shares the parent's full pages (their counts rise) and gets a copy of
+ * the used slots of its last page, when that is not full, on a page of its own.  A parent may have many children; a child is listed
+ * once, is no parent of the call, and holds no pages and length 0 before it. */
+int b200q_fork_sequences(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                         int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* parents, const int32_t* children, int n,
+                         int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes, void* stream);
+/* The held pages move to the low end of the pool: with L held pages, the k-th held page at or above L moves to the k-th free page below.
+ * Tables and counts follow; remap[num_pages] receives every held page's new number, -1 for free pages. */
+int b200q_compact_pages(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                        int64_t num_pages, int32_t* block_table, int B, int max_blocks, int page_size, int32_t* remap, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* Tensor-parallel glue (no counterpart in the reference, which is single-device): all-gather of an
  * activation shard over NVLink peer memory.  `local` [rows, row_bytes_local] is this rank's shard;

@@ -68,6 +68,25 @@ int attn_read_status(int reset, cudaStream_t stream);
 int peer_read_status(int reset, cudaStream_t stream);
 int stack_read_status(int reset, cudaStream_t stream);
 int rope_read_status(int reset, cudaStream_t stream);
+int pages_read_status(int reset, cudaStream_t stream);
+size_t reserve_workspace_impl(int B, int64_t num_pages);
+size_t copy_workspace_impl(int n, int64_t num_pages);
+size_t fork_workspace_impl(int n, int B);
+size_t compact_workspace_impl(int64_t num_pages);
+int reserve_pages_impl(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, const int32_t* lengths, const int32_t*
+                       new_tokens, int uniform, int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes,
+                       cudaStream_t stream);
+int release_sequences_impl(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* rows, int n,
+                           int B, int max_blocks, cudaStream_t stream);
+int copy_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, const int32_t* src, const
+                    int32_t* dst, int n, int64_t num_pages, int page_size, void* workspace, size_t workspace_bytes, cudaStream_t
+                    stream);
+int fork_sequences_impl(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                        int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* parents, const int32_t* children,
+                        int n, int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int compact_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                       int64_t num_pages, int32_t* block_table, int B, int max_blocks, int page_size, int32_t* remap, void* workspace,
+                       size_t workspace_bytes, cudaStream_t stream);
 int head_rope_impl(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
                    const void* k_weight, int w_dtype, float eps, const float* cos_table, const float* sin_table,
                    const int32_t* positions, int64_t table_len, int rotary_dim, int half_layout, int64_t T, int Hq, int Hkv, int D,
@@ -394,12 +413,14 @@ int b200q_device_status(int reset, void* stream) {
     const int c = peer_read_status(reset, (cudaStream_t)stream);
     const int d = stack_read_status(reset, (cudaStream_t)stream);
     const int e = rope_read_status(reset, (cudaStream_t)stream);
+    const int f = pages_read_status(reset, (cudaStream_t)stream);
     if (a < 0) return a;
     if (b < 0) return b;
     if (c < 0) return c;
     if (d < 0) return d;
     if (e < 0) return e;
-    return std::max(std::max(std::max(a, b), std::max(c, d)), e);
+    if (f < 0) return f;
+    return std::max({a, b, c, d, e, f});
 }
 
 int b200q_head_rope(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
@@ -421,6 +442,43 @@ int b200q_norm_rope_kv_append(const void* qkv, int64_t qkv_stride, const float* 
     return norm_rope_kv_append_impl(qkv, qkv_stride, cos_table, sin_table, table_len, rotary_dim, half_layout, positions, sequences,
                                     block_table, B, max_blocks, q_weight, k_weight, w_dtype, eps, q_out, kv_bits, k_pages, v_pages,
                                     k_scales, v_scales, T, Hq, Hkv, D, page_size, num_pages, group_size, dtype, (cudaStream_t)stream);
+}
+
+size_t b200q_reserve_pages_workspace_bytes(int B, int64_t num_pages) { return reserve_workspace_impl(B, num_pages); }
+size_t b200q_copy_pages_workspace_bytes(int n, int64_t num_pages) { return copy_workspace_impl(n, num_pages); }
+size_t b200q_fork_sequences_workspace_bytes(int n, int B) { return fork_workspace_impl(n, B); }
+size_t b200q_compact_pages_workspace_bytes(int64_t num_pages) { return compact_workspace_impl(num_pages); }
+int b200q_reserve_pages(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, const int32_t* lengths, const int32_t*
+                        new_tokens, int uniform, int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes, void*
+                        stream) {
+    tp_discard();
+    return reserve_pages_impl(ref_counts, num_pages, block_table, lengths, new_tokens, uniform, B, max_blocks, page_size, workspace,
+                              workspace_bytes, (cudaStream_t)stream);
+}
+int b200q_release_sequences(int32_t* ref_counts, int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* rows, int
+                            n, int B, int max_blocks, void* stream) {
+    tp_discard();
+    return release_sequences_impl(ref_counts, num_pages, block_table, lengths, rows, n, B, max_blocks, (cudaStream_t)stream);
+}
+int b200q_copy_pages(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, const int32_t* src, const
+                     int32_t* dst, int n, int64_t num_pages, int page_size, void* workspace, size_t workspace_bytes, void* stream) {
+    tp_discard();
+    return copy_pages_impl(bases0, n0, slot0, bases1, n1, slot1, src, dst, n, num_pages, page_size, workspace, workspace_bytes,
+                           (cudaStream_t)stream);
+}
+int b200q_fork_sequences(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                         int64_t num_pages, int32_t* block_table, int32_t* lengths, const int32_t* parents, const int32_t* children,
+                         int n, int B, int max_blocks, int page_size, void* workspace, size_t workspace_bytes, void* stream) {
+    tp_discard();
+    return fork_sequences_impl(bases0, n0, slot0, bases1, n1, slot1, ref_counts, num_pages, block_table, lengths, parents, children,
+                               n, B, max_blocks, page_size, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+int b200q_compact_pages(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
+                        int64_t num_pages, int32_t* block_table, int B, int max_blocks, int page_size, int32_t* remap, void*
+                        workspace, size_t workspace_bytes, void* stream) {
+    tp_discard();
+    return compact_pages_impl(bases0, n0, slot0, bases1, n1, slot1, ref_counts, num_pages, block_table, B, max_blocks, page_size,
+                              remap, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int b200q_peer_allgather(const void* local, void* const* peer_full, uint32_t* const* peer_flags, uint32_t* epoch,

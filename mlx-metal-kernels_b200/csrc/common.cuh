@@ -41,6 +41,8 @@ enum DeviceEvent : int {
     EV_PEER_WAIT = 5,         // a rank gave up waiting for a peer's shard in the peer all-gather
     EV_ROPE_POSITION = 6,     // rope + append: a position lies outside the rotary table (row left unrotated)
     EV_KV_PAGE_UNASSIGNED = 7,  // rope + append: the block table has no page for the position (nothing appended)
+    EV_PAGE_CALL = 8,         // a page operator met indices, lengths or counts it cannot take
+    EV_PAGES_EXHAUSTED = 9,   // a page operator found too few free pages (nothing changed)
 };
 
 // ---------------------------------------------------------------------------------------------

@@ -46,6 +46,15 @@ SIGNATURES = {
     "b200q_head_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _f, _vp, _vp, _vp, _i64, _i, _i, _i64, _i, _i, _i, _i, _vp]),
     "b200q_norm_rope_kv_append": (_i, [_vp, _i64, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _f, _vp, _i, _vp, _vp,
                                        _vp, _vp, _i64, _i, _i, _i, _i, _i64, _i, _i, _vp]),
+    "b200q_reserve_pages_workspace_bytes": (_sz, [_i, _i64]),
+    "b200q_copy_pages_workspace_bytes": (_sz, [_i, _i64]),
+    "b200q_fork_sequences_workspace_bytes": (_sz, [_i, _i]),
+    "b200q_compact_pages_workspace_bytes": (_sz, [_i64]),
+    "b200q_reserve_pages": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "b200q_release_sequences": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "b200q_copy_pages": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i, _i64, _i, _vp, _sz, _vp]),
+    "b200q_fork_sequences": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "b200q_compact_pages": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "b200q_attention_stage_launches": (_i, [_i, _i, _i]),
     "b200q_attention_launches": (_i, [_i, _i, _i, _i]),
     "b200q_quantize_kv": (_i, [_i, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
