@@ -50,7 +50,7 @@ const char* b200q_strerror(int code);
  * trapping: 1-5 a bounded wait (on a shared-memory barrier or on a peer's flag) ran out, 6 b200q_rope_kv_append
  * met a position outside the rotary table (the row was left unrotated), 7 it met a position whose block-table
  * entry is unassigned (nothing was appended), 8 a page operator met indices, lengths or counts that it cannot take, 9 it
- * found too few free pages.  The largest event seen is returned.  Synchronises `stream`.
+ * found too few free pages, 10 a row named an adapter that does not exist.  The largest event seen is returned.  Synchronises `stream`.
  * 0 = no event. */
 int b200q_device_status(int reset, void* stream);
 
@@ -133,6 +133,18 @@ int b200q_gate_up_swiglu(int bits, const void* x, const uint8_t* gate_codes, con
                          const void* residual_in, const void* norm_weight, int norm_w_dtype, float eps,
                          void* z_out, void* normed_out, int rows, int64_t N, int64_t K, int group_size,
                          int act_dtype, int scale_dtype, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection (no counterpart in the reference):
+ * out[t] = cast(y[t] + scaling[l] * B[l] (A[l] x[t])) with l = ids[t]; ids[t] < 0: out[t] = y[t].  x [rows, K], y and out [rows, N] (out
+ * may be y; y is, say, what b200q_qmatvec left there), A [L, R, K] and B [L, N, R], all in `dtype`; scaling [L] fp32 (NULL: 1);
+ * ranks [L] (NULL: R): adapter l uses the first ranks[l] rows of A[l] and columns of B[l], the rest is not read.  fp32 sums, and one rounding
+ * after the sum with y.  An id >= L counts as none and records event 10.  The factors, scaling, ranks and ids may be read before the
+ * previous kernel of the stream has ended when that is a kernel of this library: none of them writes to such arrays.
+ * workspace: b200q_lora_workspace_bytes(rows, R) bytes of device scratch. */
+size_t b200q_lora_workspace_bytes(int64_t rows, int R);
+int b200q_lora_add(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
+                   const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* out = cast(silu(gate) * up) on [rows, dim].  Replaces kernels/swiglu.metal and
  * kernels/fused_swiglu.metal (ops/activation_ops.py:91-153). */

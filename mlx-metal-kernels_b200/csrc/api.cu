@@ -87,6 +87,11 @@ int fork_sequences_impl(void* const* bases0, int n0, int64_t slot0, void* const*
 int compact_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* bases1, int n1, int64_t slot1, int32_t* ref_counts,
                        int64_t num_pages, int32_t* block_table, int B, int max_blocks, int page_size, int32_t* remap, void* workspace,
                        size_t workspace_bytes, cudaStream_t stream);
+int lora_read_status(int reset, cudaStream_t stream);
+size_t lora_workspace_impl(int64_t rows, int R);
+int lora_add_impl(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
+                  const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* ws, size_t ws_bytes,
+                  cudaStream_t stream);
 int head_rope_impl(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
                    const void* k_weight, int w_dtype, float eps, const float* cos_table, const float* sin_table,
                    const int32_t* positions, int64_t table_len, int rotary_dim, int half_layout, int64_t T, int Hq, int Hkv, int D,
@@ -414,13 +419,15 @@ int b200q_device_status(int reset, void* stream) {
     const int d = stack_read_status(reset, (cudaStream_t)stream);
     const int e = rope_read_status(reset, (cudaStream_t)stream);
     const int f = pages_read_status(reset, (cudaStream_t)stream);
+    const int g = lora_read_status(reset, (cudaStream_t)stream);
     if (a < 0) return a;
     if (b < 0) return b;
     if (c < 0) return c;
     if (d < 0) return d;
     if (e < 0) return e;
     if (f < 0) return f;
-    return std::max({a, b, c, d, e, f});
+    if (g < 0) return g;
+    return std::max({a, b, c, d, e, f, g});
 }
 
 int b200q_head_rope(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_weight,
@@ -442,6 +449,14 @@ int b200q_norm_rope_kv_append(const void* qkv, int64_t qkv_stride, const float* 
     return norm_rope_kv_append_impl(qkv, qkv_stride, cos_table, sin_table, table_len, rotary_dim, half_layout, positions, sequences,
                                     block_table, B, max_blocks, q_weight, k_weight, w_dtype, eps, q_out, kv_bits, k_pages, v_pages,
                                     k_scales, v_scales, T, Hq, Hkv, D, page_size, num_pages, group_size, dtype, (cudaStream_t)stream);
+}
+
+size_t b200q_lora_workspace_bytes(int64_t rows, int R) { return lora_workspace_impl(rows, R); }
+int b200q_lora_add(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
+                   const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    tp_discard();
+    return lora_add_impl(x, y, out, a, b, scaling, ranks, ids, rows, N, K, L, R, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 size_t b200q_reserve_pages_workspace_bytes(int B, int64_t num_pages) { return reserve_workspace_impl(B, num_pages); }
