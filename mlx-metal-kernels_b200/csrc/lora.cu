@@ -5,6 +5,13 @@
 // A [L, R, K] and B [L, N, R] hold the factors of L adapters, of which adapter l uses the first ranks[l] of R; x [rows, K], y and out
 // [rows, N] (out may be y).  Products are summed in fp32, the R values between the factors stay in fp32 (or in as many bits), and the
 // sum with y is rounded once.
+//
+// One launch for both products: a thread-block cluster per adapter that occurs in a block of 16 consecutive rows (the first row of its kind
+// leads; clusters of the others end at once).  The CTAs of a cluster cut K: every warp multiplies its pieces of the rows with
+// the factor A on mma.sync, straight from global memory - the order of the summands is free, so a lane takes 16 contiguous bytes of
+// a row as the k indices of two instructions.  The partial sums meet in shared memory, then through distributed shared memory
+// in every CTA; then the CTAs cut N: 32 columns per warp and round, a lane again with 8 contiguous bytes of B and 16 of y.  The values between
+// the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
 #include "common.cuh"
 
 #include <algorithm>
@@ -94,6 +101,284 @@ template <typename T> int any_size(const LoraParams& p, cudaStream_t stream) {
     return rc != B200Q_OK ? rc : launch(lora_expand_any_kernel<T>, std::min(cap, (p.rows * p.N + 255) / 256), 256, stream, p);
 }
 
+// ---- the cluster kernel: K a multiple of 8, R a multiple of 4 up to 256, 16-byte aligned factors and rows ------------------------
+constexpr int kRows = 16, kWarps = 8, kMaxRank = 256, kRankBlock = 64;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float load_remote(const float* local, uint32_t cta) {
+    uint32_t addr;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(local)), "r"(cta));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const __half*) {
+    mma_m16n8k16(d, a0, a1, a2, a3, b0, b1);
+}
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const __nv_bfloat16*) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// shared memory: partial sums of the warps, of the CTA, and the two terms of the rows between the factors
+struct LoraSmem {
+    int low_stride;           // 16-bit values per row of a term: the rank in whole steps of 16, and 8 against bank conflicts
+    size_t part, cta, hi, lo, bytes;
+};
+__host__ __device__ inline LoraSmem lora_smem(int R) {
+    LoraSmem s;
+    const int block = R < kRankBlock ? (R + 7) / 8 * 8 : kRankBlock;
+    s.low_stride = (R + 15) / 16 * 16 + 8;
+    s.part = 0;
+    s.cta = s.part + sizeof(float) * kWarps * kRows * block;
+    s.hi = s.cta + sizeof(float) * kRows * ((R + 7) / 8 * 8);
+    s.lo = s.hi + 2 * (size_t)kRows * s.low_stride;
+    s.bytes = s.lo + 2 * (size_t)kRows * s.low_stride;
+    return s;
+}
+
+// NT: rank tiles of 8 that a warp accumulates at a time
+template <typename T, int NT> __global__ void __launch_bounds__(kWarps * 32) lora_cluster_kernel(const __grid_constant__ LoraParams p, int vector_rows) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float row_scale[kRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const uint32_t cta = cluster_rank(), ctas = cluster_size();
+    const int64_t item = blockIdx.x / ctas, row0 = item / kRows * kRows;
+    const int leader = (int)(item - row0);
+    pdl_launch_dependents();
+    // ids, ranks and factors belong to no kernel that may still run (see the header): they are read before the wait
+    const int count = (int)min((int64_t)kRows, p.rows - row0);
+    const int mine = lane < count ? max(adapter_of(p, row0 + lane), -1) : -2;
+    const int id = __shfl_sync(0xFFFFFFFFu, mine, leader);
+    const unsigned members = __ballot_sync(0xFFFFFFFFu, mine == id);
+    if (__ffs(members) - 1 != leader) return;                // another row leads this adapter's; all CTAs of the cluster agree
+    if (id < 0) {
+        if (threadIdx.x == 0 && cta == 0)
+            for (int i = 0; i < count; ++i)
+                if (p.ids[row0 + i] >= p.L) atomicMax(&g_device_status, (int)EV_LORA_ADAPTER);
+        if (p.out == p.y) {
+            pdl_wait();                                      // a grid whose blocks all end before the previous kernel would hide it from the next
+            return;
+        }
+    }
+    const int rank = id < 0 ? 0 : rank_of(p, id);
+    const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
+    const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
+    const int64_t chunks = (p.K + 31) / 32, per = (chunks + ctas - 1) / ctas;
+    const int64_t c_lo = min(chunks, cta * per), c_hi = min(chunks, c_lo + per);
+    const int64_t strips = (p.N + 31) / 32;
+    // the CTA's parts of both factors on their way into L2 while the previous kernel ends
+    {
+        const int64_t lines = (c_hi - c_lo + 1) / 2;         // of two chunks
+        for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
+            const int64_t r = i / lines;
+            prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
+        }
+        const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
+        for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
+            for (int64_t i = lane; i < strip_lines; i += 32)
+                if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
+    }
+    pdl_wait();
+
+    const LoraSmem at = lora_smem(p.R);
+    float* part = reinterpret_cast<float*>(smem + at.part);
+    float* own = reinterpret_cast<float*>(smem + at.cta);
+    T* hi = reinterpret_cast<T*>(smem + at.hi);
+    T* lo = reinterpret_cast<T*>(smem + at.lo);
+    const int rank8 = (rank + 7) / 8 * 8, rank16 = (rank + 15) / 16 * 16;
+    const bool r0 = members >> g & 1u, r1 = members >> (g + 8) & 1u;
+
+    // ---- rows times A: the CTA's chunks of 32 k, dealt to its warps; a lane holds k = 8q .. 8q + 7 of a chunk ----
+    const T* x0 = reinterpret_cast<const T*>(p.x) + (row0 + g) * p.K + q * 8;
+    const T* x1 = x0 + 8 * p.K;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    constexpr int U = NT <= 2 ? 4 : NT <= 4 ? 2 : 1;         // chunks in flight
+    for (int rb = 0; rb < rank; rb += NT * 8) {
+        float acc[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+        const T* ab = a + (int64_t)(rb + g) * p.K + q * 8;
+        for (int64_t c = c_lo + warp; c < c_hi; c += kWarps * U) {
+            uint4 xa[U], xb[U], w[U][NT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t k = (c + u * kWarps) * 32;
+                const bool in = c + u * kWarps < c_hi && k + q * 8 < p.K;
+                xa[u] = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+                xb[u] = in && r1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    w[u][j] = in && rb + j * 8 + g < rank ? __ldg(reinterpret_cast<const uint4*>(ab + (int64_t)j * 8 * p.K + k)) : zero;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    mma16(acc[j], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][j].x, w[u][j].y, (const T*)nullptr);
+                    mma16(acc[j], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][j].z, w[u][j].w, (const T*)nullptr);
+                }
+        }
+        const int width = min(NT * 8, rank8 - rb);           // of this block of ranks, in whole tiles
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            if (j * 8 >= width) break;
+            float* dst = part + ((size_t)warp * kRows + g) * width + j * 8 + 2 * q;
+            dst[0] = acc[j][0];
+            dst[1] = acc[j][1];
+            dst[8 * width] = acc[j][2];
+            dst[8 * width + 1] = acc[j][3];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < kRows * width; i += kWarps * 32) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWarps; ++v) s += part[(size_t)v * kRows * width + i];
+            own[(i / width) * rank8 + rb + i % width] = s;
+        }
+        __syncthreads();
+    }
+    // ---- the CTAs' sums meet in every CTA: a warp per row, as two terms and a power of two ----
+    cluster_arrive();
+    cluster_wait();
+    for (int r = warp; r < kRows; r += kWarps) {
+        float v[kMaxRank / 32], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMaxRank / 32; ++i) {
+            v[i] = 0.0f;
+            const int k = i * 32 + lane;
+            if (k < rank && (members >> r & 1u))
+                for (uint32_t c = 0; c < ctas; ++c) v[i] += load_remote(own + r * rank8 + k, c);
+            top = fmaxf(top, fabsf(v[i]));
+        }
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        // the largest value to [2^13, 2^14); the factor and its inverse are exact
+        const int e = top > 0.0f && top < INFINITY ? min(126, 13 + 127 - (int)(__float_as_uint(top) >> 23)) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < kMaxRank / 32; ++i) {
+            const int k = i * 32 + lane;
+            if (k >= rank16) continue;
+            const float t = v[i] * up;
+            const T h = from_f32<T>(t);
+            const float rest = t - to_f32(h);
+            hi[r * at.low_stride + k] = h;
+            lo[r * at.low_stride + k] = from_f32<T>(fabsf(rest) < INFINITY ? rest : 0.0f);
+        }
+        if (lane == 0) row_scale[r] = down * (p.scaling && id >= 0 ? p.scaling[id] : 1.0f);
+    }
+    cluster_arrive();                                        // nobody reads this CTA's sums any more: waited for at the end
+    __syncthreads();
+
+    // ---- times B: 32 columns per warp and round.  Instruction j's column n is base + 8 (n / 2) + 2 j + n % 2, so that a lane's results
+    //      are columns base + 8 q .. + 7 of rows g and g + 8 ----
+    const T* y = reinterpret_cast<const T*>(p.y);
+    T* out = reinterpret_cast<T*>(p.out);
+    for (int64_t s = (int64_t)cta * kWarps + warp; s < strips; s += (int64_t)ctas * kWarps) {
+        const int64_t n0 = s * 32, mine_n = n0 + q * 8;
+        float acc[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+        const int64_t col = n0 + (g >> 1) * 8 + (g & 1);
+        constexpr int KS = NT <= 2 ? 1 : NT <= 4 ? 2 : 4;    // steps of 16 ranks in flight
+        for (int k0 = 0; k0 < rank16; k0 += 16 * KS) {
+            uint2 w[KS][4];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = k0 + ks * 16 + q * 4;
+                    w[ks][j] = make_uint2(0u, 0u);
+                    if (k < rank && col + 2 * j < p.N) {
+                        w[ks][j] = __ldg(reinterpret_cast<const uint2*>(b + (col + 2 * j) * p.R + k));
+                        if (k + 4 > rank) {                  // values behind the rank are not the adapter's
+                            if (k + 1 >= rank) w[ks][j].x &= 0xFFFFu;
+                            if (k + 2 >= rank) w[ks][j].y = 0u;
+                            else if (k + 3 >= rank) w[ks][j].y &= 0xFFFFu;
+                        }
+                    }
+                }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int k = k0 + ks * 16 + q * 4;
+                if (k0 + ks * 16 >= rank16) break;
+                const uint2 h0 = *reinterpret_cast<const uint2*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const uint2*>(hi + (g + 8) * at.low_stride + k);
+                const uint2 l0 = *reinterpret_cast<const uint2*>(lo + g * at.low_stride + k), l1 = *reinterpret_cast<const uint2*>(lo + (g + 8) * at.low_stride + k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    mma16(acc[j], h0.x, h1.x, h0.y, h1.y, w[ks][j].x, w[ks][j].y, (const T*)nullptr);
+                    mma16(acc[j], l0.x, l1.x, l0.y, l1.y, w[ks][j].x, w[ks][j].y, (const T*)nullptr);
+                }
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = g + 8 * half;
+            if (!(members >> r & 1u) || mine_n >= p.N) continue;
+            const int64_t at_y = (row0 + r) * p.N + mine_n;
+            const float f = row_scale[r];
+            if (vector_rows) {                               // N a multiple of 8: whole pieces
+                const uint4 u = *reinterpret_cast<const uint4*>(y + at_y);
+                const T* e = reinterpret_cast<const T*>(&u);
+                T o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = id < 0 ? e[i] : from_f32<T>(fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e[i])));
+                *reinterpret_cast<uint4*>(out + at_y) = *reinterpret_cast<const uint4*>(o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (mine_n + i < p.N) {
+                        const T e = y[at_y + i];
+                        out[at_y + i] = id < 0 ? e : from_f32<T>(fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e)));
+                    }
+            }
+        }
+    }
+    cluster_wait();
+}
+
+template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
+    int ctas = tuning_get("lora.cluster");
+    if (ctas <= 0) ctas = 8;
+    if (p.rows > INT32_MAX / ctas) return B200Q_ERR_UNSUPPORTED;
+    const size_t smem = lora_smem(p.R).bytes;
+    void (*kernel)(const LoraParams, int) = p.R <= 16 ? lora_cluster_kernel<T, 2> : p.R <= 32 ? lora_cluster_kernel<T, 4> : lora_cluster_kernel<T, 8>;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tuning_get("no_pdl") ? 1 : 2;
+    const int vector_rows = p.N % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) & 15u) == 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
+}
+bool cluster_takes(const LoraParams& p) {
+    return p.K % 8 == 0 && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;
+}
+
 }  // namespace
 
 size_t lora_workspace_impl(int64_t rows, int R) { return rows <= 0 || R <= 0 ? 0 : 4 * (size_t)rows * (size_t)R; }
@@ -105,6 +390,7 @@ int lora_add_impl(const void* x, const void* y, void* out, const void* a, const 
     if (rows <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0 || !is_act_dtype(dtype)) return B200Q_ERR_BAD_ARG;
     if (ws == nullptr || ws_bytes < lora_workspace_impl(rows, R)) return B200Q_ERR_WORKSPACE;
     const LoraParams p = {x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R};
+    if (cluster_takes(p)) return dtype == B200Q_F16 ? cluster_form<__half>(p, stream) : cluster_form<__nv_bfloat16>(p, stream);
     return dtype == B200Q_F16 ? any_size<__half>(p, stream) : any_size<__nv_bfloat16>(p, stream);
 }
 
