@@ -12,8 +12,9 @@
 // quantised from the rounded values with the cache's rule (see stack.cu).
 //
 // Bound by HBM for prompts and by latency for a few tokens.  A head is taken by D/16 lanes, so that a lane has two 16-byte pieces
-// of it: pieces l and l + D/16, which are the two halves of eight pairs in the half layout over whole heads.  Four
-// heads of one token per lane keep eight loads in flight and share the token's cos / sin and the norm's weights.
+// of it: pieces l and l + D/16, which are the two halves of eight pairs in the half layout over whole heads.  One head per
+// lane while all fit the GPU at once; else two (RUN) of one token, which share the token's cos / sin and the norm's weights, with four blocks
+// per SM: for 8185 tokens of 48 heads with norms 48 us, against 56 with four heads and 68 with one.
 #include "common.cuh"
 
 #include <algorithm>
@@ -24,7 +25,6 @@ B200Q_DEFINE_STATUS_WORD(rope_read_status)
 
 namespace {
 
-constexpr int kRun = 4;          // heads of one token and kind that a group of lanes takes
 constexpr int kThreads = 256;
 
 enum HeadKind : int { KIND_Q = 0, KIND_K = 1, KIND_V = 2 };
@@ -44,7 +44,7 @@ struct RopeParams {
     void* codes[3];               // k and v pages at KIND_K, KIND_V
     __half* scales[3];
     int64_t T, table_len, num_pages;
-    int heads[3], runs[3];        // heads per kind, and groups of kRun of them
+    int heads[3], runs[3];        // heads per kind, and groups of RUN of them
     int B, max_blocks, P, D, R, G, w_dtype;
     float eps;
 };
@@ -110,31 +110,31 @@ template <int CACHE> __device__ __forceinline__ uint32_t kv_code(float v, float 
 }
 
 // D a power of two from 32 to 256, R a multiple of 16, groups of whole pieces, everything aligned to 16 bytes.
-template <typename T, int LAYOUT, int CACHE>
-__global__ void __launch_bounds__(kThreads) rope_heads_kernel(const __grid_constant__ RopeParams p, int log_lanes, int64_t units) {
+template <typename T, int LAYOUT, int CACHE, int RUN>
+__global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ? 3 : 4) rope_heads_kernel(const __grid_constant__ RopeParams p, int log_lanes, uint32_t units) {
     pdl_launch_dependents();
     pdl_wait();
     const int lanes = 1 << log_lanes;                        // lanes of a head: D / 16
     const int l = threadIdx.x & (lanes - 1);
-    const int64_t unit = (int64_t)blockIdx.x * (kThreads >> log_lanes) + (threadIdx.x >> log_lanes);
+    const uint32_t unit = blockIdx.x * (kThreads >> log_lanes) + (threadIdx.x >> log_lanes);
     const bool live = unit < units;
-    const int per_token = p.runs[0] + p.runs[1] + p.runs[2];
-    const int64_t t = live ? unit / per_token : 0;
-    int run = live ? (int)(unit - t * per_token) : 0;
+    const uint32_t per_token = p.runs[0] + p.runs[1] + p.runs[2], token = live ? unit / per_token : 0;
+    const int64_t t = token;
+    int run = live ? (int)(unit - token * per_token) : 0;
     int kind = KIND_Q;
     if (run >= p.runs[0]) { run -= p.runs[0]; kind = KIND_K; }
     if (kind == KIND_K && run >= p.runs[1]) { run -= p.runs[1]; kind = KIND_V; }
-    const int h0 = run * kRun;
-    const int count = live ? min(kRun, p.heads[kind] - h0) : 0;
+    const int h0 = run * RUN;
+    const int count = live ? min(RUN, p.heads[kind] - h0) : 0;
     const int d0 = l * 8, d1 = (l + lanes) * 8;              // first dimension of the lane's two pieces
 
     const T* src = reinterpret_cast<const T*>(p.in[kind]) + t * p.in_token[kind] + (int64_t)h0 * p.in_head[kind];
-    uint4 x0[kRun], x1[kRun], o0[kRun], o1[kRun];            // o: the partners of the pieces, where another lane owns them
+    uint4 x0[RUN], x1[RUN], o0[RUN], o1[RUN];            // o: the partners of the pieces, where another lane owns them
     const int half = p.R / 2;
     const bool turns = kind != KIND_V;
     const int partner0 = d0 < half ? d0 + half : d0 - half, partner1 = d1 < half ? d1 + half : d1 - half;
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < RUN; ++j) {
         x0[j] = x1[j] = o0[j] = o1[j] = make_uint4(0u, 0u, 0u, 0u);
         if (j < count) {
             const T* row = src + j * p.in_head[kind];
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) rope_heads_kernel(const __grid_const
     if (LAYOUT == HALF_PART) __syncwarp();                   // in place: nobody stores before the partners are loaded
 
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < RUN; ++j) {
         float a[8], b[8];
         unpack8(x0[j], a, (const T*)nullptr);
         unpack8(x1[j], b, (const T*)nullptr);
@@ -276,9 +276,23 @@ __global__ void __launch_bounds__(kThreads) rope_heads_kernel(const __grid_const
                 const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
                 const int64_t row = row_index * p.heads[kind] + h0 + j;
                 auto store = [&](const float (&v)[8], float scale, int d) {
+                    // rint(v / scale) through the reciprocal, as in the page quantiser (stack.cu): the same integer unless the quotient
+                    // lies within 2^-14 of a tie or is not finite; those pieces are divided
+                    constexpr float magic = 12582912.0f + (CACHE == CACHE_Q8 ? 128.0f : 8.0f);
+                    const float inv = __fdividef(1.0f, scale);
                     uint32_t c[8];
+                    float far = 0.0f, sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
+                    for (int i = 0; i < 8; ++i) {
+                        const float r = fmaf(v[i], inv, magic);
+                        far = fmaxf(far, fabsf(fmaf(v[i], inv, magic - r)));
+                        sum += v[i] * 0.0f;                  // not zero when a value is not finite
+                        c[i] = __float_as_uint(r) & 0xFFu;
+                    }
+                    if (!(sum == 0.0f) || !(far <= 0.4999f) || !(scale < 1e30f)) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
+                    }
                     uint8_t* codes = reinterpret_cast<uint8_t*>(p.codes[kind]);
                     if (CACHE == CACHE_Q8)
                         *reinterpret_cast<uint2*>(codes + row * p.D + d) =
@@ -404,12 +418,22 @@ int dispatch(RopeParams& p, bool half_layout, cudaStream_t stream) {
     if (pow2 && p.R % 16 == 0 && groups && aligned16(p)) {
         int log_lanes = 1;
         while ((16 << log_lanes) < p.D) ++log_lanes;
-        for (int i = 0; i < 3; ++i) p.runs[i] = (p.heads[i] + kRun - 1) / kRun;
-        const int64_t units = p.T * (p.runs[0] + p.runs[1] + p.runs[2]), per_block = kThreads >> log_lanes;
-        const int64_t blocks = (units + per_block - 1) / per_block;
-        if (!half_layout) return launch(rope_heads_kernel<T, INTERLEAVED, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
-        if (p.R == p.D) return launch(rope_heads_kernel<T, HALF_WHOLE, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
-        return launch(rope_heads_kernel<T, HALF_PART, CACHE>, blocks, kThreads, 0, stream, p, log_lanes, units);
+        // one head per group of lanes while all of them fit the GPU at once (the shortest chain), else two (RUN)
+        const int64_t all = p.T * ((int64_t)p.heads[0] + p.heads[1] + p.heads[2]), per_block = kThreads >> log_lanes;
+        const int run = all <= (int64_t)sm_count() * 4 * per_block ? 1 : 2;
+        for (int i = 0; i < 3; ++i) p.runs[i] = (p.heads[i] + run - 1) / run;
+        const int64_t units = p.T * ((int64_t)p.runs[0] + p.runs[1] + p.runs[2]), blocks = (units + per_block - 1) / per_block;
+        if (units <= INT32_MAX) {
+            const uint32_t n = (uint32_t)units;
+            if (run == 1) {
+                if (!half_layout) return launch(rope_heads_kernel<T, INTERLEAVED, CACHE, 1>, blocks, kThreads, 0, stream, p, log_lanes, n);
+                if (p.R == p.D) return launch(rope_heads_kernel<T, HALF_WHOLE, CACHE, 1>, blocks, kThreads, 0, stream, p, log_lanes, n);
+                return launch(rope_heads_kernel<T, HALF_PART, CACHE, 1>, blocks, kThreads, 0, stream, p, log_lanes, n);
+            }
+            if (!half_layout) return launch(rope_heads_kernel<T, INTERLEAVED, CACHE, 2>, blocks, kThreads, 0, stream, p, log_lanes, n);
+            if (p.R == p.D) return launch(rope_heads_kernel<T, HALF_WHOLE, CACHE, 2>, blocks, kThreads, 0, stream, p, log_lanes, n);
+            return launch(rope_heads_kernel<T, HALF_PART, CACHE, 2>, blocks, kThreads, 0, stream, p, log_lanes, n);
+        }
     }
     const int64_t units = p.T * (p.heads[0] + p.heads[1] + p.heads[2]);
     return launch(rope_any_kernel<T, CACHE>, (units + kAnyWarps - 1) / kAnyWarps, kAnyWarps * 32, sizeof(float) * kAnyWarps * p.D, stream, p,
