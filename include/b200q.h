@@ -72,7 +72,7 @@ int b200q_device_status(int reset, void* stream);
  *   "attn.force_simple"  1 = always the one-warp-per-head attention kernel
  *   "peer.spin_limit", "tp.spin_limit"   flag probes after which b200q_peer_allgather / the wait of an exchange fused
  *                        into a kernel gives up and records event 5 (default 2^22; tests shorten it)
- *   "lora.cluster"       CTAs per cluster of b200q_lora_add: 1, 2, 4 or 8 (default: by rows)
+ *   "lora.cluster", "lora.span"     CTAs per cluster of b200q_lora_add (1, 2, 4, 8 or 16) and leading rows per cluster (default: by rows)
  *   "no_pdl"             1 = launch without programmatic dependent launch */
 int b200q_set_tuning(const char* key, int value);
 
@@ -137,7 +137,7 @@ int b200q_gate_up_swiglu(int bits, const void* x, const uint8_t* gate_codes, con
 
 /* Low-rank adapters of many requests beside a shared projection (no counterpart in the reference):
  * out[t] = cast(y[t] + scaling[l] * B[l] (A[l] x[t])) with l = ids[t]; ids[t] < 0: out[t] = y[t].  x [rows, K], y and out [rows, N] (out
- * may be y; y is, say, what b200q_qmatvec left there), A [L, R, K] and B [L, N, R], all in `dtype`; scaling [L] fp32 (NULL: 1);
+ * may be y, and y NULL: 0), A [L, R, K] and B [L, N, R], all in `dtype`; scaling [L] fp32 (NULL: 1);
  * ranks [L] (NULL: R): adapter l uses the first ranks[l] rows of A[l] and columns of B[l], the rest is not read.  fp32 sums, and one rounding
  * after the sum with y.  An id >= L counts as none and records event 10.  The factors, scaling, ranks and ids may be read before the
  * previous kernel of the stream has ended when that is a kernel of this library: none of them writes to such arrays.

@@ -6,15 +6,20 @@
 // [rows, N] (out may be y).  Products are summed in fp32, the R values between the factors stay in fp32 (or in as many bits), and the
 // sum with y is rounded once.
 //
-// One launch for both products: a thread-block cluster per adapter that occurs in a block of 16 consecutive rows (the first row of its kind
-// leads; clusters of the others end at once).  The CTAs of a cluster cut K: every warp multiplies its pieces of the rows with
-// the factor A on mma.sync, straight from global memory - the order of the summands is free, so a lane takes 16 contiguous bytes of
-// a row as the k indices of two instructions.  The partial sums meet in shared memory, then through distributed shared memory
-// in every CTA; then the CTAs cut N: 32 columns per warp and round, a lane again with 8 contiguous bytes of B and 16 of y.  The values between
-// the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
+// One launch for both products: a thread-block cluster per adapter and up to 16 of the rows that use it.  Rows are looked at in windows of 256;
+// of the rows of an adapter in a window every sixteenth leads a group (its cluster works, the others' end at once).  The CTAs of a
+// cluster cut K: every warp multiplies its pieces of the rows with the factor A on mma.sync, straight from global memory - the
+// order of the summands is free, so a lane takes 16 contiguous bytes of a row as the k indices of two instructions.  The partial sums
+// meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp and round, a
+// lane with contiguous bytes of B again and 16 bytes of y, the next round's loads in flight during this one's products.  The values
+// between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
+//
+// Bound by latency for a few rows (a chain of ids, first factor, two meetings, second factor), by L2 for prompts, whose groups of 16 rows read
+// both factors again.
 #include "common.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200q {
 
@@ -24,7 +29,7 @@ namespace {
 
 struct LoraParams {
     const void* x;            // [rows, K]
-    const void* y;            // [rows, N]
+    const void* y;            // [rows, N] or null: 0
     void* out;                // [rows, N]
     const void* a;            // [L, R, K]
     const void* b;            // [L, N, R]
@@ -69,7 +74,7 @@ template <typename T> __global__ void __launch_bounds__(256) lora_expand_any_ker
     for (int64_t it = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; it < items; it += threads) {
         const int64_t row = it / p.N, n = it - row * p.N;
         const int id = adapter_of(p, row);
-        const float y = to_f32(reinterpret_cast<const T*>(p.y)[it]);
+        const T y = p.y ? reinterpret_cast<const T*>(p.y)[it] : from_f32<T>(0.0f);
         float s = 0.0f;
         if (id >= 0) {
             const T* b = reinterpret_cast<const T*>(p.b) + ((int64_t)id * p.N + n) * p.R;
@@ -78,7 +83,7 @@ template <typename T> __global__ void __launch_bounds__(256) lora_expand_any_ker
             for (int r = 0; r < rank; ++r) s = fmaf(to_f32(b[r]), low[r], s);
             if (p.scaling) s *= p.scaling[id];
         }
-        reinterpret_cast<T*>(p.out)[it] = id < 0 ? reinterpret_cast<const T*>(p.y)[it] : from_f32<T>(y + s);
+        reinterpret_cast<T*>(p.out)[it] = id < 0 ? y : from_f32<T>(to_f32(y) + s);
     }
 }
 
@@ -102,7 +107,8 @@ template <typename T> int any_size(const LoraParams& p, cudaStream_t stream) {
 }
 
 // ---- the cluster kernel: K a multiple of 8, R a multiple of 4 up to 256, 16-byte aligned factors and rows ------------------------
-constexpr int kRows = 16, kWarps = 8, kMaxRank = 256, kRankBlock = 64;
+constexpr int kRows = 16, kWarps = 8, kMaxRank = 256, kRankBlock = 64, kMaxCtas = 16;
+constexpr int kWindow = kWarps * 32;      // rows that one group may come from: an id per thread
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -135,15 +141,28 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// zeros for all but the first n (> 0 or not) values of a piece
+__device__ __forceinline__ uint32_t keep2(uint32_t v, int n) { return n >= 2 ? v : n == 1 ? v & 0xFFFFu : 0u; }
+__device__ __forceinline__ void keep_ranks(uint2& v, int n) {
+    v.x = keep2(v.x, n);
+    v.y = keep2(v.y, n - 2);
+}
+__device__ __forceinline__ void keep_ranks(uint4& v, int n) {
+    v.x = keep2(v.x, n);
+    v.y = keep2(v.y, n - 2);
+    v.z = keep2(v.z, n - 4);
+    v.w = keep2(v.w, n - 6);
+}
+
 // shared memory: partial sums of the warps, of the CTA, and the two terms of the rows between the factors
 struct LoraSmem {
-    int low_stride;           // 16-bit values per row of a term: the rank in whole steps of 16, and 8 against bank conflicts
+    int low_stride;           // 16-bit values per row of a term: the rank in whole steps of 32, and 8 against bank conflicts
     size_t part, cta, hi, lo, bytes;
 };
 __host__ __device__ inline LoraSmem lora_smem(int R) {
     LoraSmem s;
     const int block = R < kRankBlock ? (R + 7) / 8 * 8 : kRankBlock;
-    s.low_stride = (R + 15) / 16 * 16 + 8;
+    s.low_stride = (R + 31) / 32 * 32 + 8;
     s.part = 0;
     s.cta = s.part + sizeof(float) * kWarps * kRows * block;
     s.hi = s.cta + sizeof(float) * kRows * ((R + 7) / 8 * 8);
@@ -152,215 +171,293 @@ __host__ __device__ inline LoraSmem lora_smem(int R) {
     return s;
 }
 
-// NT: rank tiles of 8 that a warp accumulates at a time
-template <typename T, int NT> __global__ void __launch_bounds__(kWarps * 32) lora_cluster_kernel(const __grid_constant__ LoraParams p, int vector_rows) {
+// A round's part of B and of y, loaded ahead: STEPS pieces of B for each of its four tiles.
+template <int STEPS, typename PIECE> struct Strip {
+    PIECE w[STEPS][4];
+    uint4 y[2];
+};
+
+// NT: rank tiles of 8 that a warp accumulates at a time.  NT 2 takes ranks by 16 (8 bytes of B per lane), NT 4 and 8 by 32 (16 bytes).
+template <typename T, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_kernel(const __grid_constant__ LoraParams p, int span, int vector_rows) {
+    using Piece = std::conditional_t<NT <= 2, uint2, uint4>;
+    constexpr int kPer = sizeof(Piece) / 2;                  // ranks in a lane's piece
+    constexpr int kStep = 4 * kPer, kSteps = NT <= 4 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float row_scale[kRows];
+    __shared__ unsigned match[kWindow / 32];
+    __shared__ int row_of[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t cta = cluster_rank(), ctas = cluster_size();
-    const int64_t item = blockIdx.x / ctas, row0 = item / kRows * kRows;
-    const int leader = (int)(item - row0);
-    pdl_launch_dependents();
-    // ids, ranks and factors belong to no kernel that may still run (see the header): they are read before the wait
-    const int count = (int)min((int64_t)kRows, p.rows - row0);
-    const int mine = lane < count ? max(adapter_of(p, row0 + lane), -1) : -2;
-    const int id = __shfl_sync(0xFFFFFFFFu, mine, leader);
-    const unsigned members = __ballot_sync(0xFFFFFFFFu, mine == id);
-    if (__ffs(members) - 1 != leader) return;                // another row leads this adapter's; all CTAs of the cluster agree
-    if (id < 0) {
-        if (threadIdx.x == 0 && cta == 0)
-            for (int i = 0; i < count; ++i)
-                if (p.ids[row0 + i] >= p.L) atomicMax(&g_device_status, (int)EV_LORA_ADAPTER);
-        if (p.out == p.y) {
-            pdl_wait();                                      // a grid whose blocks all end before the previous kernel would hide it from the next
-            return;
-        }
-    }
-    const int rank = id < 0 ? 0 : rank_of(p, id);
-    const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
-    const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
-    const int64_t chunks = (p.K + 31) / 32, per = (chunks + ctas - 1) / ctas;
-    const int64_t c_lo = min(chunks, cta * per), c_hi = min(chunks, c_lo + per);
-    const int64_t strips = (p.N + 31) / 32;
-    // the CTA's parts of both factors on their way into L2 while the previous kernel ends
-    {
-        const int64_t lines = (c_hi - c_lo + 1) / 2;         // of two chunks
-        for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
-            const int64_t r = i / lines;
-            prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
-        }
-        const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
-        for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
-            for (int64_t i = lane; i < strip_lines; i += 32)
-                if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
-    }
-    pdl_wait();
-
     const LoraSmem at = lora_smem(p.R);
     float* part = reinterpret_cast<float*>(smem + at.part);
     float* own = reinterpret_cast<float*>(smem + at.cta);
     T* hi = reinterpret_cast<T*>(smem + at.hi);
     T* lo = reinterpret_cast<T*>(smem + at.lo);
-    const int rank8 = (rank + 7) / 8 * 8, rank16 = (rank + 15) / 16 * 16;
-    const bool r0 = members >> g & 1u, r1 = members >> (g + 8) & 1u;
-
-    // ---- rows times A: the CTA's chunks of 32 k, dealt to its warps; a lane holds k = 8q .. 8q + 7 of a chunk ----
-    const T* x0 = reinterpret_cast<const T*>(p.x) + (row0 + g) * p.K + q * 8;
-    const T* x1 = x0 + 8 * p.K;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    constexpr int U = NT <= 2 ? 4 : NT <= 4 ? 2 : 1;         // chunks in flight
-    for (int rb = 0; rb < rank; rb += NT * 8) {
-        float acc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-        const T* ab = a + (int64_t)(rb + g) * p.K + q * 8;
-        for (int64_t c = c_lo + warp; c < c_hi; c += kWarps * U) {
-            uint4 xa[U], xb[U], w[U][NT];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t k = (c + u * kWarps) * 32;
-                const bool in = c + u * kWarps < c_hi && k + q * 8 < p.K;
-                xa[u] = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-                xb[u] = in && r1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    w[u][j] = in && rb + j * 8 + g < rank ? __ldg(reinterpret_cast<const uint4*>(ab + (int64_t)j * 8 * p.K + k)) : zero;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    mma16(acc[j], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][j].x, w[u][j].y, (const T*)nullptr);
-                    mma16(acc[j], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][j].z, w[u][j].w, (const T*)nullptr);
-                }
-        }
-        const int width = min(NT * 8, rank8 - rb);           // of this block of ranks, in whole tiles
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            if (j * 8 >= width) break;
-            float* dst = part + ((size_t)warp * kRows + g) * width + j * 8 + 2 * q;
-            dst[0] = acc[j][0];
-            dst[1] = acc[j][1];
-            dst[8 * width] = acc[j][2];
-            dst[8 * width + 1] = acc[j][3];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < kRows * width; i += kWarps * 32) {
-            float s = 0.0f;
-#pragma unroll
-            for (int v = 0; v < kWarps; ++v) s += part[(size_t)v * kRows * width + i];
-            own[(i / width) * rank8 + rb + i % width] = s;
-        }
-        __syncthreads();
-    }
-    // ---- the CTAs' sums meet in every CTA: a warp per row, as two terms and a power of two ----
-    cluster_arrive();
-    cluster_wait();
-    for (int r = warp; r < kRows; r += kWarps) {
-        float v[kMaxRank / 32], top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kMaxRank / 32; ++i) {
-            v[i] = 0.0f;
-            const int k = i * 32 + lane;
-            if (k < rank && (members >> r & 1u))
-                for (uint32_t c = 0; c < ctas; ++c) v[i] += load_remote(own + r * rank8 + k, c);
-            top = fmaxf(top, fabsf(v[i]));
-        }
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        // the largest value to [2^13, 2^14); the factor and its inverse are exact
-        const int e = top > 0.0f && top < INFINITY ? min(126, 13 + 127 - (int)(__float_as_uint(top) >> 23)) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < kMaxRank / 32; ++i) {
-            const int k = i * 32 + lane;
-            if (k >= rank16) continue;
-            const float t = v[i] * up;
-            const T h = from_f32<T>(t);
-            const float rest = t - to_f32(h);
-            hi[r * at.low_stride + k] = h;
-            lo[r * at.low_stride + k] = from_f32<T>(fabsf(rest) < INFINITY ? rest : 0.0f);
-        }
-        if (lane == 0) row_scale[r] = down * (p.scaling && id >= 0 ? p.scaling[id] : 1.0f);
-    }
-    cluster_arrive();                                        // nobody reads this CTA's sums any more: waited for at the end
-    __syncthreads();
-
-    // ---- times B: 32 columns per warp and round.  Instruction j's column n is base + 8 (n / 2) + 2 j + n % 2, so that a lane's results
-    //      are columns base + 8 q .. + 7 of rows g and g + 8 ----
     const T* y = reinterpret_cast<const T*>(p.y);
     T* out = reinterpret_cast<T*>(p.out);
-    for (int64_t s = (int64_t)cta * kWarps + warp; s < strips; s += (int64_t)ctas * kWarps) {
-        const int64_t n0 = s * 32, mine_n = n0 + q * 8;
-        float acc[4][4];
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int64_t chunks = (p.K + 31) / 32, per = (chunks + ctas - 1) / ctas;
+    const int64_t c_lo = min(chunks, cta * per), c_hi = min(chunks, c_lo + per);
+    const int64_t strips = (p.N + 31) / 32;
+    pdl_launch_dependents();
+    bool waited = false;
+
+    const int64_t first = (int64_t)(blockIdx.x / ctas) * span;
+    for (int64_t lead = first; lead < min(p.rows, first + span); ++lead) {
+        // ---- the group that this row leads.  ids, ranks and factors belong to no kernel that may still run (see the header): they are
+        //      read before the wait ----
+        const int64_t row0 = lead / kWindow * kWindow;
+        const int id = max(adapter_of(p, lead), -1);
+        const bool same = row0 + threadIdx.x < p.rows && max(adapter_of(p, row0 + threadIdx.x), -1) == id;
+        const unsigned vote = __ballot_sync(0xFFFFFFFFu, same);
+        if (lane == 0) match[warp] = vote;
+        __syncthreads();
+        const int me = (int)(lead - row0);
+        int before = 0, mine = 0;                            // rows of the adapter ahead of the leader, and ahead of this thread's row
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-        const int64_t col = n0 + (g >> 1) * 8 + (g & 1);
-        constexpr int KS = NT <= 2 ? 1 : NT <= 4 ? 2 : 4;    // steps of 16 ranks in flight
-        for (int k0 = 0; k0 < rank16; k0 += 16 * KS) {
-            uint2 w[KS][4];
+        for (int i = 0; i < kWindow / 32; ++i) {
+            const int c = __popc(match[i]);
+            if (i < me / 32) before += c;
+            if (i < warp) mine += c;
+        }
+        before += __popc(match[me / 32] & ((1u << (me & 31)) - 1u));
+        mine += __popc(vote & ((1u << lane) - 1u));
+        if (threadIdx.x < kRows) row_of[threadIdx.x] = -1;
+        if (before % kRows != 0) {                           // all CTAs of the cluster agree
+            __syncthreads();
+            continue;
+        }
+        __syncthreads();
+        if (same && mine >= before && mine < before + kRows) row_of[mine - before] = threadIdx.x;
+        const int rank = id < 0 ? 0 : rank_of(p, id);
+        const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
+        const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
+        if (!waited) {
+            // the CTA's parts of both factors on their way into L2 while the previous kernel ends
+            const int64_t lines = (c_hi - c_lo + 1) / 2;     // of two chunks
+            for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
+                const int64_t r = i / lines;
+                prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
+            }
+            const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
+            for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
+                for (int64_t i = lane; i < strip_lines; i += 32)
+                    if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
+            pdl_wait();
+            waited = true;
+        }
+        __syncthreads();
+        if (id < 0) {
+            if (cta == 0 && threadIdx.x < kRows && row_of[threadIdx.x] >= 0 && p.ids[row0 + row_of[threadIdx.x]] >= p.L)
+                atomicMax(&g_device_status, (int)EV_LORA_ADAPTER);
+            if (p.out == p.y) {
+                __syncthreads();
+                continue;
+            }
+        }
+        const int rank8 = (rank + 7) / 8 * 8, rank16 = (rank + 15) / 16 * 16;
+        const int t0 = row_of[g], t1 = row_of[g + 8];
+        const bool r0 = t0 >= 0, r1 = t1 >= 0;
+
+        // a round's loads: instruction j's column n is 32 s + 8 (n / 2) + 2 j + n % 2, so that a lane's results are columns 32 s + 8 q .. + 7
+        // of rows g and g + 8
+        auto load_b = [&](Piece (&w)[kSteps][4], int64_t s, int k0) {
+            const int64_t col = s * 32 + (g >> 1) * 8 + (g & 1);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int st = 0; st < kSteps; ++st)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int k = k0 + ks * 16 + q * 4;
-                    w[ks][j] = make_uint2(0u, 0u);
-                    if (k < rank && col + 2 * j < p.N) {
-                        w[ks][j] = __ldg(reinterpret_cast<const uint2*>(b + (col + 2 * j) * p.R + k));
-                        if (k + 4 > rank) {                  // values behind the rank are not the adapter's
-                            if (k + 1 >= rank) w[ks][j].x &= 0xFFFFu;
-                            if (k + 2 >= rank) w[ks][j].y = 0u;
-                            else if (k + 3 >= rank) w[ks][j].y &= 0xFFFFu;
+                    const int k = k0 + st * kStep + q * kPer;
+                    Piece v = {};
+                    if (k < rank && col + 2 * j < p.N) v = __ldg(reinterpret_cast<const Piece*>(b + (col + 2 * j) * p.R + k));
+                    w[st][j] = v;
+                }
+        };
+        auto load_strip = [&](Strip<kSteps, Piece>& strip, int64_t s) {
+            load_b(strip.w, s, 0);
+            const int64_t n = s * 32 + q * 8;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int t = half ? t1 : t0;
+                strip.y[half] = zero;
+                if (y == nullptr || t < 0 || n >= p.N) continue;
+                const T* src = y + (row0 + t) * p.N + n;
+                if (vector_rows) {
+                    strip.y[half] = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    T e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = n + i < p.N ? src[i] : from_f32<T>(0.0f);
+                    strip.y[half] = *reinterpret_cast<const uint4*>(e);
+                }
+            }
+        };
+        const int64_t s_first = (int64_t)cta * kWarps + warp, s_step = (int64_t)ctas * kWarps;
+        Strip<kSteps, Piece> strip;
+        if (s_first < strips) load_strip(strip, s_first);
+
+        // ---- rows times A: the CTA's chunks of 32 k, dealt to its warps; a lane holds k = 8q .. 8q + 7 of a chunk ----
+        const T* x0 = reinterpret_cast<const T*>(p.x) + (row0 + max(t0, 0)) * p.K + q * 8;
+        const T* x1 = reinterpret_cast<const T*>(p.x) + (row0 + max(t1, 0)) * p.K + q * 8;
+        constexpr int U = NT <= 2 ? 4 : NT <= 4 ? 2 : 1;     // chunks in flight
+        for (int rb = 0; rb < rank; rb += NT * 8) {
+            float acc[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+            const T* ab = a + (int64_t)(rb + g) * p.K + q * 8;
+            for (int64_t c = c_lo + warp; c < c_hi; c += kWarps * U) {
+                uint4 xa[U], xb[U], w[U][NT];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t k = (c + u * kWarps) * 32;
+                    const bool in = c + u * kWarps < c_hi && k + q * 8 < p.K;
+                    xa[u] = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+                    xb[u] = in && r1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        w[u][j] = in && rb + j * 8 + g < rank ? __ldg(reinterpret_cast<const uint4*>(ab + (int64_t)j * 8 * p.K + k)) : zero;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        mma16(acc[j], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][j].x, w[u][j].y, (const T*)nullptr);
+                        mma16(acc[j], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][j].z, w[u][j].w, (const T*)nullptr);
+                    }
+            }
+            const int width = min(NT * 8, rank8 - rb);       // of this block of ranks, in whole tiles
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (j * 8 >= width) break;
+                float* dst = part + ((size_t)warp * kRows + g) * width + j * 8 + 2 * q;
+                dst[0] = acc[j][0];
+                dst[1] = acc[j][1];
+                dst[8 * width] = acc[j][2];
+                dst[8 * width + 1] = acc[j][3];
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < kRows * width; i += kWarps * 32) {
+                float s = 0.0f;
+#pragma unroll
+                for (int v = 0; v < kWarps; ++v) s += part[(size_t)v * kRows * width + i];
+                own[(i / width) * rank8 + rb + i % width] = s;
+            }
+            __syncthreads();
+        }
+        // ---- the CTAs' sums meet in every CTA: a warp per row, as two terms and a power of two ----
+        cluster_arrive();
+        cluster_wait();
+        for (int r = warp; r < kRows; r += kWarps) {
+            const bool used = row_of[r] >= 0;
+            float v[kMaxRank / 32], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kMaxRank / 32; ++i) {
+                v[i] = 0.0f;
+                const int k = i * 32 + lane;
+                if (i * 32 < rank && used) {
+                    float u[kMaxCtas];
+#pragma unroll
+                    for (int c = 0; c < kMaxCtas; ++c) u[c] = c < ctas && k < rank ? load_remote(own + r * rank8 + k, c) : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < kMaxCtas; ++c) v[i] += u[c];
+                }
+                top = fmaxf(top, fabsf(v[i]));
+            }
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            // the largest value to [2^13, 2^14); the factor and its inverse are exact
+            const int e = top > 0.0f && top < INFINITY ? min(126, 13 + 127 - (int)(__float_as_uint(top) >> 23)) : 0;
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+            for (int i = 0; i < kMaxRank / 32; ++i) {
+                const int k = i * 32 + lane;
+                if (k >= (rank16 + 31) / 32 * 32) continue;
+                const float t = v[i] * up;
+                const T h = from_f32<T>(t);
+                const float rest = t - to_f32(h);
+                hi[r * at.low_stride + k] = h;
+                lo[r * at.low_stride + k] = from_f32<T>(fabsf(rest) < INFINITY ? rest : 0.0f);
+            }
+            if (lane == 0) row_scale[r] = down * (p.scaling && id >= 0 ? p.scaling[id] : 1.0f);
+        }
+        cluster_arrive();                                    // nobody reads this CTA's sums any more: waited for at the end
+        __syncthreads();
+
+        // ---- times B ----
+        for (int64_t s = s_first; s < strips; s += s_step) {
+            Strip<kSteps, Piece> next;
+            if (s + s_step < strips) load_strip(next, s + s_step);
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+            auto multiply = [&](Piece (&w)[kSteps][4], int k0) {
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) {
+                    const int k = k0 + st * kStep + q * kPer;
+                    if (k0 + st * kStep >= rank) break;
+                    const Piece h0 = *reinterpret_cast<const Piece*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const Piece*>(hi + (g + 8) * at.low_stride + k);
+                    const Piece l0 = *reinterpret_cast<const Piece*>(lo + g * at.low_stride + k), l1 = *reinterpret_cast<const Piece*>(lo + (g + 8) * at.low_stride + k);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        Piece v = w[st][j];
+                        if (k + kPer > rank) keep_ranks(v, rank - k);      // values behind the rank are not the adapter's
+                        mma16(acc[j], h0.x, h1.x, h0.y, h1.y, v.x, v.y, (const T*)nullptr);
+                        mma16(acc[j], l0.x, l1.x, l0.y, l1.y, v.x, v.y, (const T*)nullptr);
+                        if constexpr (kPer == 8) {
+                            mma16(acc[j], h0.z, h1.z, h0.w, h1.w, v.z, v.w, (const T*)nullptr);
+                            mma16(acc[j], l0.z, l1.z, l0.w, l1.w, v.z, v.w, (const T*)nullptr);
                         }
                     }
                 }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int k = k0 + ks * 16 + q * 4;
-                if (k0 + ks * 16 >= rank16) break;
-                const uint2 h0 = *reinterpret_cast<const uint2*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const uint2*>(hi + (g + 8) * at.low_stride + k);
-                const uint2 l0 = *reinterpret_cast<const uint2*>(lo + g * at.low_stride + k), l1 = *reinterpret_cast<const uint2*>(lo + (g + 8) * at.low_stride + k);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mma16(acc[j], h0.x, h1.x, h0.y, h1.y, w[ks][j].x, w[ks][j].y, (const T*)nullptr);
-                    mma16(acc[j], l0.x, l1.x, l0.y, l1.y, w[ks][j].x, w[ks][j].y, (const T*)nullptr);
-                }
+            };
+            multiply(strip.w, 0);
+            for (int k0 = kSteps * kStep; k0 < rank; k0 += kSteps * kStep) {
+                load_b(strip.w, s, k0);
+                multiply(strip.w, k0);
             }
-        }
+            const int64_t n = s * 32 + q * 8;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = g + 8 * half;
-            if (!(members >> r & 1u) || mine_n >= p.N) continue;
-            const int64_t at_y = (row0 + r) * p.N + mine_n;
-            const float f = row_scale[r];
-            if (vector_rows) {                               // N a multiple of 8: whole pieces
-                const uint4 u = *reinterpret_cast<const uint4*>(y + at_y);
-                const T* e = reinterpret_cast<const T*>(&u);
+            for (int half = 0; half < 2; ++half) {
+                const int t = half ? t1 : t0;
+                if (t < 0 || n >= p.N) continue;
+                const float f = row_scale[g + 8 * half];
+                const T* e = reinterpret_cast<const T*>(&strip.y[half]);
                 T o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[i] = id < 0 ? e[i] : from_f32<T>(fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e[i])));
-                *reinterpret_cast<uint4*>(out + at_y) = *reinterpret_cast<const uint4*>(o);
-            } else {
+                T* dst = out + (row0 + t) * p.N + n;
+                if (vector_rows) {
+                    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (mine_n + i < p.N) {
-                        const T e = y[at_y + i];
-                        out[at_y + i] = id < 0 ? e : from_f32<T>(fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e)));
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        if (n + i < p.N) dst[i] = o[i];
+                }
             }
+            strip = next;
         }
+        cluster_wait();                                      // also: no CTA overwrites its sums for the next row while another reads them
+        __syncthreads();
     }
-    cluster_wait();
+    if (!waited) pdl_wait();                                 // a grid whose blocks all end early would hide the previous kernel from the next
 }
 
 template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
     int ctas = tuning_get("lora.cluster");
     if (ctas <= 0) ctas = 8;
-    if (p.rows > INT32_MAX / ctas) return B200Q_ERR_UNSUPPORTED;
+    // leading rows per cluster: one, until the clusters of all rows are several times what the GPU holds
+    int64_t span = tuning_get("lora.span");
+    if (span <= 0) span = std::max<int64_t>(1, p.rows * ctas / ((int64_t)sm_count() * 8));
+    const int64_t clusters = (p.rows + span - 1) / span;
+    if (clusters > INT32_MAX / ctas || span > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
     const size_t smem = lora_smem(p.R).bytes;
-    void (*kernel)(const LoraParams, int) = p.R <= 16 ? lora_cluster_kernel<T, 2> : p.R <= 32 ? lora_cluster_kernel<T, 4> : lora_cluster_kernel<T, 8>;
+    void (*kernel)(const LoraParams, int, int) = p.R <= 16 || p.R % 8 != 0 || ((uintptr_t)p.b & 15u) != 0 ? lora_cluster_kernel<T, 2>
+                                               : p.R <= 32                                               ? lora_cluster_kernel<T, 4>
+                                                                                                         : lora_cluster_kernel<T, 8>;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return B200Q_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.rows * ctas));
+    cfg.gridDim = dim3((unsigned)(clusters * ctas));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -373,7 +470,7 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     cfg.attrs = attr;
     cfg.numAttrs = tuning_get("no_pdl") ? 1 : 2;
     const int vector_rows = p.N % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) & 15u) == 0;
-    return cudaLaunchKernelEx(&cfg, kernel, p, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, p, (int)span, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
 }
 bool cluster_takes(const LoraParams& p) {
     return p.K % 8 == 0 && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;
@@ -386,7 +483,7 @@ size_t lora_workspace_impl(int64_t rows, int R) { return rows <= 0 || R <= 0 ? 0
 int lora_add_impl(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
                   const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* ws, size_t ws_bytes,
                   cudaStream_t stream) {
-    if (x == nullptr || y == nullptr || out == nullptr || a == nullptr || b == nullptr || ids == nullptr) return B200Q_ERR_BAD_ARG;
+    if (x == nullptr || out == nullptr || a == nullptr || b == nullptr || ids == nullptr) return B200Q_ERR_BAD_ARG;
     if (rows <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0 || !is_act_dtype(dtype)) return B200Q_ERR_BAD_ARG;
     if (ws == nullptr || ws_bytes < lora_workspace_impl(rows, R)) return B200Q_ERR_WORKSPACE;
     const LoraParams p = {x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R};

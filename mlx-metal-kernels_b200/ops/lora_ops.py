@@ -63,7 +63,7 @@ def _launch(x2d, y2d, out2d, adapters, ids, device):
     scaling, ranks = _cabi.contiguous(adapters.scaling), _cabi.contiguous(adapters.ranks)
     lib = _cabi.load()
     ws = torch.empty(max(16, lib.b200q_lora_workspace_bytes(rows, R)), dtype=torch.uint8, device=device)
-    _cabi.check(lib.b200q_lora_add(x2d.data_ptr(), y2d.data_ptr(), out2d.data_ptr(), a.data_ptr(), b.data_ptr(), _cabi.ptr(scaling),
+    _cabi.check(lib.b200q_lora_add(x2d.data_ptr(), _cabi.ptr(y2d), out2d.data_ptr(), a.data_ptr(), b.data_ptr(), _cabi.ptr(scaling),
                                    _cabi.ptr(ranks), ids.data_ptr(), rows, b.shape[1], K, L, R, _cabi.dtype_code(x2d.dtype), ws.data_ptr(),
                                    ws.numel(), _cabi.stream()), "b200q_lora_add")
 
@@ -86,8 +86,13 @@ def lora_add(y, x, adapters: LoraAdapters, adapter_ids):
 
 
 def lora_quantized_linear(x, w, scales, zeros, adapters: LoraAdapters, adapter_ids, *, bits=4, group_size=32, residual=None, backend="auto"):
-    """``quantized_linear`` with the adapter of every row: [B,K] / [B,S,K] -> N features.  The shared product is rounded to x.dtype (with
-    ``residual`` [.., N]: cast(residual + cast(W x)), as in the MLP block), then the adapters are added as in ``lora_add``."""
+    """``quantized_linear`` with the adapter of every row: [B,K] / [B,S,K] -> N features.  The adapters' part (with ``residual`` [.., N]: its
+    sum with that) is rounded to x.dtype and goes into the shared product as the residual row does in the MLP block:
+    y = cast(cast(residual + scaling * B (A x)) + cast(W x)).  In this order the product's weights are on their way while the adapters
+    are computed."""
+    out = _cabi.host().lora_linear(bits, x, w, scales, zeros, group_size, backend, adapters, adapter_ids, residual)
+    if out is not None:
+        return out
     x2d, shape = _normalize_hidden_input(x)
     _, out_dim = _validate_quantized_linear_shapes(x2d, w, scales, zeros, bits=bits, group_size=group_size, name="lora_quantized_linear")
     _resolve_matvec_backend(backend, "lora_quantized_linear")
@@ -99,6 +104,9 @@ def lora_quantized_linear(x, w, scales, zeros, adapters: LoraAdapters, adapter_i
         return torch.empty((*shape[:-1], out_dim), dtype=x.dtype, device=device)
     with _cabi.on_device(device):
         x2d = _cabi.contiguous(x2d)
-        y = matvec_rows(bits, x2d, w, scales, zeros, group_size, None if residual is None else residual.reshape(-1, out_dim))
-        _launch(x2d, y, y, adapters, ids, device)
+        if residual is not None:
+            residual = _cabi.contiguous(residual.reshape(-1, out_dim).to(x.dtype))
+        low = torch.empty((x2d.shape[0], out_dim), dtype=x.dtype, device=device)
+        _launch(x2d, residual, low, adapters, ids, device)
+        y = matvec_rows(bits, x2d, w, scales, zeros, group_size, low)
     return _restore_hidden_output(y, shape)

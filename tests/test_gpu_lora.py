@@ -80,18 +80,19 @@ def test_lora_add(cuda, rows, N, K, L, R, dtype, spread):
 @pytest.mark.parametrize("rows,N,K,G", [(1, 512, 1024, 64), (6, 1003, 96, 32), (40, 256, 512, 64)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_quantized_linear(cuda, bits, rows, N, K, G, dtype):
-    """The shared product is quantized_linear's own, bit for bit."""
+    """The adapters' rows, rounded, are the residual of quantized_linear's own product, bit for bit."""
     w, s, z = (t.to(cuda) for t in synth.quantized_weight(N, K, bits, G, seed=N))
     x = synth.activations((rows, K), 2).to(dtype).to(cuda)
     ids = torch.tensor([(i % 4) - 1 for i in range(rows)], dtype=torch.int32, device=cuda)
     ad = make(3, 16, K, N, dtype, cuda, 3)
     base = mlp_ops.quantized_linear(x, w, s, z, bits=bits, group_size=G)
     got = lora.lora_quantized_linear(x, w, s, z, ad, ids, bits=bits, group_size=G)
-    assert torch.equal(got, lora.lora_add(base, x, ad, ids))
-    check(got, base, x, ad, ids)
+    low = lora.lora_add(torch.zeros_like(base), x, ad, ids)
+    check(low, torch.zeros_like(base), x, ad, ids)
+    assert torch.equal(got, (low.float() + base.float()).to(dtype))
     res = synth.activations((rows, N), 5).to(dtype).to(cuda)
     with_res = lora.lora_quantized_linear(x, w, s, z, ad, ids, bits=bits, group_size=G, residual=res)
-    check(with_res, (res.float() + base.float()).to(dtype), x, ad, ids)
+    assert torch.equal(with_res, (lora.lora_add(res, x, ad, ids).float() + base.float()).to(dtype))
 
 
 def test_shapes_of_prompts(cuda):
