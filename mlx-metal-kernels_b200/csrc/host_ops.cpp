@@ -55,6 +55,21 @@ int (*p_head_rope)(const void*, const void*, void*, void*, const int64_t*, const
 int (*p_append)(const void*, int64_t, const float*, const float*, int64_t, int, int, const int32_t*, const int32_t*, const int32_t*, int, int,
                 const void*, const void*, int, float, void*, int, void*, void*, void*, void*, int64_t, int, int, int, int, int64_t, int, int,
                 void*) = nullptr;
+size_t (*p_lora_ws)(int64_t, int) = nullptr;
+int (*p_lora)(const void*, const void*, void*, const void*, const void*, const float*, const int32_t*, const int32_t*, int64_t, int64_t, int64_t,
+              int, int, int, void*, size_t, void*) = nullptr;
+size_t (*p_reserve_ws)(int, int64_t) = nullptr;
+size_t (*p_copy_ws)(int, int64_t) = nullptr;
+size_t (*p_fork_ws)(int, int) = nullptr;
+size_t (*p_compact_ws)(int64_t) = nullptr;
+int (*p_reserve)(int32_t*, int64_t, int32_t*, const int32_t*, const int32_t*, int, int, int, int, void*, size_t, void*) = nullptr;
+int (*p_release)(int32_t*, int64_t, int32_t*, int32_t*, const int32_t*, int, int, int, void*) = nullptr;
+int (*p_copy_pages)(void* const*, int, int64_t, void* const*, int, int64_t, const int32_t*, const int32_t*, int, int64_t, int, void*, size_t,
+                    void*) = nullptr;
+int (*p_fork)(void* const*, int, int64_t, void* const*, int, int64_t, int32_t*, int64_t, int32_t*, int32_t*, const int32_t*, const int32_t*, int,
+              int, int, int, void*, size_t, void*) = nullptr;
+int (*p_compact)(void* const*, int, int64_t, void* const*, int, int64_t, int32_t*, int64_t, int32_t*, int, int, int, int32_t*, void*, size_t,
+                 void*) = nullptr;
 
 constexpr int kMaxDevices = 64;
 constexpr int kErrUnsupported = -2, kErrWorkspace = -4;      // B200Q_ERR_*
@@ -523,6 +538,211 @@ PyObject* norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return rc == 0 ? THPVariable_Wrap(std::move(out)) : none();
 }
 
+PyObject *s_a, *s_b, *s_scaling, *s_ranks, *s_kz, *s_vz;
+
+// lora_linear(bits, x, w, scales, zeros, group_size, backend, adapters, adapter_ids, residual or None) -> y or None
+PyObject* lora_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    int64_t bits, group;
+    if (p_lora == nullptr || n_args != 10 || !as_int(a[0], &bits) || !as_int(a[5], &group) || group <= 0 || (bits != 4 && bits != 8)) return none();
+    if (!one_of(a[6], {"cuda", "auto", "metal", "metal_tiled", "metal_parallel"}) || safe_mode()) return none();
+    const Tensor *x = as_tensor(a[1]), *ids = as_tensor(a[8]), *res = as_tensor(a[9]);
+    const int dev = current_device_of(x);
+    if (dev < 0 || ids == nullptr || (res == nullptr && a[9] != Py_None) || !x->is_contiguous() || !act_dtype(x->scalar_type()) ||
+        (x->dim() != 2 && x->dim() != 3))
+        return none();
+    const int64_t n = x->dim(), K = x->size(n - 1), rows = n == 2 ? x->size(0) : x->size(0) * x->size(1);
+    Matrix m;
+    if (rows <= 0 || rows > INT32_MAX || K <= 0 || !matrix(m, a[2], a[3], a[4], (int)bits, K, group, dev)) return none();
+    if (!on(*ids, dev) || ids->scalar_type() != at::kInt || ids->sizes() != x->sizes().slice(0, n - 1)) return none();
+    if (res != nullptr && (!on(*res, dev) || res->scalar_type() != x->scalar_type() || res->dim() != n || res->numel() != rows * m.n ||
+                           res->sizes().slice(0, n - 1) != x->sizes().slice(0, n - 1)))
+        return none();
+    Attr fa(a[7], s_a), fb(a[7], s_b), fs(a[7], s_scaling), fr(a[7], s_ranks);
+    if (fa.o == nullptr || fb.o == nullptr || fs.o == nullptr || fr.o == nullptr) return none();
+    const Tensor *la = as_tensor(fa.o), *lb = as_tensor(fb.o), *ls = as_tensor(fs.o), *lr = as_tensor(fr.o);
+    if (la == nullptr || lb == nullptr || (ls == nullptr && fs.o != Py_None) || (lr == nullptr && fr.o != Py_None)) return none();
+    if (!on(*la, dev) || !on(*lb, dev) || la->scalar_type() != x->scalar_type() || lb->scalar_type() != x->scalar_type() || la->dim() != 3 ||
+        lb->dim() != 3 || la->size(2) != K || lb->size(1) != m.n || la->size(0) != lb->size(0) || la->size(1) != lb->size(2) || la->numel() == 0 ||
+        la->size(0) > INT32_MAX || la->size(1) > INT32_MAX)
+        return none();
+    const int64_t L = la->size(0), R = la->size(1);
+    if (ls != nullptr && (!on(*ls, dev) || ls->scalar_type() != at::kFloat || ls->dim() != 1 || ls->size(0) != L)) return none();
+    if (lr != nullptr && (!on(*lr, dev) || lr->scalar_type() != at::kInt || lr->dim() != 1 || lr->size(0) != L)) return none();
+    const int act = dtype_code(x->scalar_type());
+    void* st = stream_of(dev);
+    // one scratch block: the adapters' rows [rows, N], and what the two calls ask for
+    const int64_t low_bytes = (rows * m.n * 2 + 255) / 256 * 256;
+    const size_t lora_bytes = p_lora_ws(rows, (int)R), mat_bytes = p_scratch_bytes((int)rows, K, act), more = std::max(lora_bytes, mat_bytes);
+    Tensor scratch = empty({low_bytes + (int64_t)more}, at::kByte, dev);
+    uint8_t* low = static_cast<uint8_t*>(scratch.mutable_data_ptr());
+    std::vector<int64_t> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = m.n;
+    Tensor y = empty(shape, x->scalar_type(), dev);
+    if (p_lora(x->const_data_ptr(), ptr(res), low, la->const_data_ptr(), lb->const_data_ptr(), ls == nullptr ? nullptr : f32(ls), i32(lr), i32(ids),
+               rows, m.n, K, (int)L, (int)R, act, low + low_bytes, more, st) != 0)
+        return none();
+    p_scratch_next(mat_bytes ? low + low_bytes : nullptr, mat_bytes);
+    const int rc = p_qmatvec((int)bits, x->const_data_ptr(), codes(m.w), ptr(m.s), ptr(m.z), low, y.mutable_data_ptr(), (int)rows, m.n, K, (int)group,
+                             act, dtype_code(m.s->scalar_type()), st);
+    return rc == 0 ? THPVariable_Wrap(std::move(y)) : none();
+}
+
+// ---- pages of the caches of all layers ----
+// The tensors of one call: two groups of one shape each, (codes or values) and scales.
+struct Layers {
+    std::vector<void*> base[2];
+    const Tensor* like[2] = {nullptr, nullptr};
+    int64_t slot[2] = {0, 0};
+    std::vector<PyObject*> owned;      // attributes, released with the struct: the caches hold them meanwhile
+    ~Layers() {
+        for (PyObject* o : owned) Py_DECREF(o);
+    }
+};
+bool add_layer_tensor(Layers& l, int group, PyObject* o, int dev) {
+    const Tensor* t = as_tensor(o);
+    if (t == nullptr || !on(*t, dev) || t->dim() != 4 || t->numel() == 0) return false;
+    const Tensor*& like = l.like[group];
+    if (like == nullptr) like = t;
+    else if (t->sizes() != like->sizes() || t->scalar_type() != like->scalar_type()) return false;
+    l.base[group].push_back(const_cast<void*>(t->const_data_ptr()));
+    return true;
+}
+// caches: a list or tuple of pairs of tensors or of quantised caches, all of one kind
+bool layers_of(Layers& l, PyObject* caches, int64_t num_pages, int64_t page_size, int dev) {
+    if (!PyList_Check(caches) && !PyTuple_Check(caches)) return false;
+    PyObject** items = PySequence_Fast_ITEMS(caches);
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(caches);
+    if (n <= 0 || n > 4096) return false;
+    l.owned.reserve(6 * n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* c = items[i];
+        if (PyTuple_CheckExact(c)) {
+            if (PyTuple_GET_SIZE(c) != 2 || !add_layer_tensor(l, 0, PyTuple_GET_ITEM(c, 0), dev) || !add_layer_tensor(l, 0, PyTuple_GET_ITEM(c, 1), dev))
+                return false;
+            continue;
+        }
+        const struct { PyObject* name; int group; } want[6] = {{s_kq, 0}, {s_vq, 0}, {s_ks, 1}, {s_vs, 1}, {s_kz, -1}, {s_vz, -1}};
+        for (const auto& w : want) {
+            PyObject* o = PyObject_GetAttr(c, w.name);
+            if (o == nullptr) {
+                PyErr_Clear();
+                return false;
+            }
+            l.owned.push_back(o);
+            if (w.group < 0 ? o != Py_None : !add_layer_tensor(l, w.group, o, dev)) return false;
+        }
+    }
+    if (l.like[1] != nullptr && l.base[1].size() != l.base[0].size()) return false;
+    for (int g = 0; g < 2; ++g) {
+        const Tensor* t = l.like[g];
+        if (t == nullptr) continue;
+        if (t->size(0) != num_pages || t->size(1) != page_size) return false;
+        l.slot[g] = t->size(2) * t->size(3) * (int64_t)t->element_size();
+    }
+    return l.like[0] != nullptr;
+}
+int32_t* w32(const Tensor* t) { return static_cast<int32_t*>(t->mutable_data_ptr()); }
+bool index_vector(const Tensor* t, int dev) { return t != nullptr && on(*t, dev) && t->dim() == 1 && t->scalar_type() == at::kInt && t->size(0) <= INT32_MAX; }
+// counts, page size, block table and (where asked for) lengths of a page call
+struct Pool {
+    const Tensor *refs, *table, *lengths;
+    int64_t pages, P, B, blocks;
+    int dev;
+};
+bool pool_of(Pool& p, PyObject* refs, PyObject* page_size, PyObject* table, PyObject* lengths) {
+    p.refs = as_tensor(refs);
+    p.table = as_tensor(table);
+    p.lengths = lengths == nullptr ? nullptr : as_tensor(lengths);
+    p.dev = current_device_of(p.refs);
+    if (p.dev < 0 || !index_vector(p.refs, p.dev) || !as_int(page_size, &p.P) || p.P <= 0 || p.P > INT32_MAX || p.refs->size(0) <= 0) return false;
+    if (p.table == nullptr || !on(*p.table, p.dev) || p.table->dim() != 2 || p.table->scalar_type() != at::kInt || p.table->numel() == 0) return false;
+    p.pages = p.refs->size(0);
+    p.B = p.table->size(0);
+    p.blocks = p.table->size(1);
+    if (p.B > INT32_MAX || p.blocks > INT32_MAX) return false;
+    return lengths == nullptr || (index_vector(p.lengths, p.dev) && p.lengths->size(0) == p.B);
+}
+PyObject* done(int rc) {
+    if (rc != 0) return none();
+    Py_RETURN_TRUE;
+}
+
+// reserve_pages(ref_counts, page_size, block_table, lengths, new tokens: int or tensor) -> True or None
+PyObject* reserve_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    Pool p;
+    if (p_reserve == nullptr || n_args != 5 || !pool_of(p, a[0], a[1], a[2], a[3])) return none();
+    int64_t uniform = 0;
+    const Tensor* per_row = as_tensor(a[4]);
+    if (per_row != nullptr ? !index_vector(per_row, p.dev) || per_row->size(0) != p.B : !as_int(a[4], &uniform) || uniform < 0 || uniform > INT32_MAX)
+        return none();
+    const size_t bytes = p_reserve_ws((int)p.B, p.pages);
+    Tensor ws = empty({(int64_t)bytes}, at::kByte, p.dev);
+    return done(p_reserve(w32(p.refs), p.pages, w32(p.table), i32(p.lengths), i32(per_row), (int)uniform, (int)p.B, (int)p.blocks, (int)p.P,
+                          ws.mutable_data_ptr(), bytes, stream_of(p.dev)));
+}
+
+// release_sequences(ref_counts, page_size, block_table, lengths, rows) -> True or None
+PyObject* release_sequences(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    Pool p;
+    if (p_release == nullptr || n_args != 5 || !pool_of(p, a[0], a[1], a[2], a[3])) return none();
+    const Tensor* rows = as_tensor(a[4]);
+    if (!index_vector(rows, p.dev) || rows->size(0) == 0) return none();
+    return done(p_release(w32(p.refs), p.pages, w32(p.table), w32(p.lengths), i32(rows), (int)rows->size(0), (int)p.B, (int)p.blocks, stream_of(p.dev)));
+}
+
+// fork_sequences(caches, ref_counts, page_size, block_table, lengths, parents, children) -> True or None
+PyObject* fork_sequences(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    Pool p;
+    if (p_fork == nullptr || n_args != 7 || !pool_of(p, a[1], a[2], a[3], a[4])) return none();
+    const Tensor *parents = as_tensor(a[5]), *children = as_tensor(a[6]);
+    Layers l;
+    if (!index_vector(parents, p.dev) || !index_vector(children, p.dev) || parents->size(0) == 0 || parents->size(0) != children->size(0) ||
+        !layers_of(l, a[0], p.pages, p.P, p.dev))
+        return none();
+    const int n = (int)parents->size(0);
+    const size_t bytes = p_fork_ws(n, (int)p.B);
+    Tensor ws = empty({(int64_t)bytes}, at::kByte, p.dev);
+    return done(p_fork(l.base[0].data(), (int)l.base[0].size(), l.slot[0], l.base[1].data(), (int)l.base[1].size(), l.slot[1], w32(p.refs), p.pages,
+                       w32(p.table), w32(p.lengths), i32(parents), i32(children), n, (int)p.B, (int)p.blocks, (int)p.P, ws.mutable_data_ptr(), bytes,
+                       stream_of(p.dev)));
+}
+
+// compact_pages(caches, ref_counts, page_size, block_table) -> remap or None
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    Pool p;
+    Layers l;
+    if (p_compact == nullptr || n_args != 4 || !pool_of(p, a[1], a[2], a[3], nullptr) || !layers_of(l, a[0], p.pages, p.P, p.dev)) return none();
+    const size_t bytes = p_compact_ws(p.pages);
+    Tensor ws = empty({(int64_t)bytes}, at::kByte, p.dev), remap = empty({p.pages}, at::kInt, p.dev);
+    const int rc = p_compact(l.base[0].data(), (int)l.base[0].size(), l.slot[0], l.base[1].data(), (int)l.base[1].size(), l.slot[1], w32(p.refs), p.pages,
+                             w32(p.table), (int)p.B, (int)p.blocks, (int)p.P, w32(&remap), ws.mutable_data_ptr(), bytes, stream_of(p.dev));
+    return rc == 0 ? THPVariable_Wrap(std::move(remap)) : none();
+}
+
+// copy_pages(caches, src, dst) -> True or None
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (p_copy_pages == nullptr || n_args != 3) return none();
+    const Tensor *src = as_tensor(a[1]), *dst = as_tensor(a[2]);
+    const int dev = current_device_of(src);
+    if (dev < 0 || !index_vector(src, dev) || !index_vector(dst, dev) || src->size(0) == 0 || src->size(0) != dst->size(0) ||
+        (!PyList_Check(a[0]) && !PyTuple_Check(a[0])) || PySequence_Fast_GET_SIZE(a[0]) == 0)
+        return none();
+    // the pool's size is the first tensor's
+    PyObject* first = PySequence_Fast_ITEMS(a[0])[0];
+    Attr quantised(PyTuple_CheckExact(first) ? Py_None : first, s_kq);
+    const Tensor* t = PyTuple_CheckExact(first) && PyTuple_GET_SIZE(first) == 2 ? as_tensor(PyTuple_GET_ITEM(first, 0))
+                      : quantised.o != nullptr                                 ? as_tensor(quantised.o)
+                                                                                : nullptr;
+    Layers l;
+    if (t == nullptr || t->dim() != 4 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX || !layers_of(l, a[0], t->size(0), t->size(1), dev))
+        return none();
+    const int n = (int)src->size(0);
+    const size_t bytes = p_copy_ws(n, t->size(0));
+    Tensor ws = empty({(int64_t)bytes}, at::kByte, dev);
+    return done(p_copy_pages(l.base[0].data(), (int)l.base[0].size(), l.slot[0], l.base[1].data(), (int)l.base[1].size(), l.slot[1], i32(src), i32(dst), n,
+                             t->size(0), (int)t->size(1), ws.mutable_data_ptr(), bytes, stream_of(dev)));
+}
+
 // bind({symbol: address}): the C ABI functions to call
 PyObject* bind(PyObject*, PyObject* table) {
     const struct { const char* name; void** slot; } want[] = {
@@ -532,6 +752,11 @@ PyObject* bind(PyObject*, PyObject* table) {
         {"b200q_paged_gqa_decode", (void**)&p_attn}, {"b200q_paged_gqa_decode_window", (void**)&p_attn_window},
         {"b200q_paged_fp16_gqa_workspace_bytes", (void**)&p_plain_ws}, {"b200q_paged_fp16_gqa_decode", (void**)&p_plain_attn},
         {"b200q_paged_fp16_gqa_decode_checked", (void**)&p_plain_checked},
+        {"b200q_lora_workspace_bytes", (void**)&p_lora_ws}, {"b200q_lora_add", (void**)&p_lora},
+        {"b200q_reserve_pages_workspace_bytes", (void**)&p_reserve_ws}, {"b200q_copy_pages_workspace_bytes", (void**)&p_copy_ws},
+        {"b200q_fork_sequences_workspace_bytes", (void**)&p_fork_ws}, {"b200q_compact_pages_workspace_bytes", (void**)&p_compact_ws},
+        {"b200q_reserve_pages", (void**)&p_reserve}, {"b200q_release_sequences", (void**)&p_release},
+        {"b200q_copy_pages", (void**)&p_copy_pages}, {"b200q_fork_sequences", (void**)&p_fork}, {"b200q_compact_pages", (void**)&p_compact},
         {"b200q_head_rope", (void**)&p_head_rope}, {"b200q_norm_rope_kv_append", (void**)&p_append},
         {"b200q_quantize_kv_pair", (void**)&p_quant_pair}, {"b200q_dequantize_kv_pair", (void**)&p_dequant_pair},
     };
@@ -564,6 +789,12 @@ PyMethodDef methods[] = {
     {"dequantize_kv", FAST(dequantize_kv), METH_FASTCALL, nullptr},
     {"head_rope", FAST(head_rope), METH_FASTCALL, nullptr},
     {"norm_rope_append", FAST(norm_rope_append), METH_FASTCALL, nullptr},
+    {"lora_linear", FAST(lora_linear), METH_FASTCALL, nullptr},
+    {"reserve_pages", FAST(reserve_pages), METH_FASTCALL, nullptr},
+    {"release_sequences", FAST(release_sequences), METH_FASTCALL, nullptr},
+    {"fork_sequences", FAST(fork_sequences), METH_FASTCALL, nullptr},
+    {"compact_pages", FAST(compact_pages), METH_FASTCALL, nullptr},
+    {"copy_pages", FAST(copy_pages), METH_FASTCALL, nullptr},
     {"plain_attention", FAST(plain_attention), METH_FASTCALL, nullptr},
     {"paged_attention", FAST(paged_attention), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
@@ -576,6 +807,7 @@ PyMODINIT_FUNC PyInit__b200q_host() {
     const struct { const char* name; PyObject** slot; } names[] = {
         {"bits", &s_bits}, {"group_size", &s_group_size}, {"original_page_shape", &s_shape},
         {"k_pages_q", &s_kq}, {"v_pages_q", &s_vq}, {"k_scales", &s_ks}, {"v_scales", &s_vs}, {"block_table", &s_bt}, {"lengths", &s_len},
+        {"a", &s_a}, {"b", &s_b}, {"scaling", &s_scaling}, {"ranks", &s_ranks}, {"k_zeros", &s_kz}, {"v_zeros", &s_vz},
     };
     for (const auto& n : names)
         if ((*n.slot = PyUnicode_InternFromString(n.name)) == nullptr) return nullptr;

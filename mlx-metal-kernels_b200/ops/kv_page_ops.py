@@ -127,6 +127,8 @@ def reserve_pages(pool: PagePool, block_table, lengths, new_tokens) -> None:
     """Pages for the next tokens: sequence b gets a page for every unassigned block of the positions ``lengths[b]`` to ``lengths[b] +
     new - 1``, new being ``new_tokens`` (an int) or ``new_tokens[b]`` (int32 [B]).  ``block_table`` and the pool change in place; ``lengths`` is
     left to the caller."""
+    if _cabi.host().reserve_pages(pool.ref_counts, pool.page_size, block_table, lengths, new_tokens):
+        return
     B, max_blocks = _check_table(pool, block_table, lengths)
     uniform, per_row = 0, None
     if isinstance(new_tokens, torch.Tensor):
@@ -149,6 +151,8 @@ def reserve_pages(pool: PagePool, block_table, lengths, new_tokens) -> None:
 def release_sequences(pool: PagePool, block_table, lengths, rows) -> None:
     """The sequences ``rows`` (int32 [n]) end: the counts of their pages fall by one, their block-table rows become -1, their lengths 0.
     A row listed twice is released once; a row that is empty stays so."""
+    if _cabi.host().release_sequences(pool.ref_counts, pool.page_size, block_table, lengths, rows):
+        return
     B, max_blocks = _check_table(pool, block_table, lengths)
     rows = _indices(rows, "rows")
     device = _cabi.require_cuda(pool.ref_counts, block_table, lengths, rows)
@@ -163,6 +167,8 @@ def release_sequences(pool: PagePool, block_table, lengths, rows) -> None:
 def copy_pages(caches, src_pages, dst_pages) -> None:
     """Page ``src_pages[i]`` to page ``dst_pages[i]`` (int32 [n]) in every tensor of ``caches``: a PagedQuantizedKVCache, a pair (K_pages,
     V_pages), or a list of them, one per layer.  Destinations must differ from one another and from all sources."""
+    if _cabi.host().copy_pages(caches, src_pages, dst_pages):
+        return
     src, dst = _indices(src_pages, "src_pages"), _indices(dst_pages, "dst_pages")
     if src.shape != dst.shape:
         raise ValueError(f"src_pages and dst_pages must have one shape, got {tuple(src.shape)}, {tuple(dst.shape)}")
@@ -182,6 +188,8 @@ def fork_sequences(caches, pool: PagePool, block_table, lengths, parents, childr
     """Sequence ``children[i]`` continues as ``parents[i]`` does now (int32 [n]): it shares the parent's full pages and gets the used slots of
     its last page, when that is not full, on a page of its own, in every layer of ``caches``.  A parent may have many children; a child must
     be empty (``release_sequences``), listed once, and no parent of the call.  Pages reserved behind the parent's length stay its own."""
+    if _cabi.host().fork_sequences(caches, pool.ref_counts, pool.page_size, block_table, lengths, parents, children):
+        return
     B, max_blocks = _check_table(pool, block_table, lengths)
     parents, children = _indices(parents, "parents"), _indices(children, "children")
     if parents.shape != children.shape:
@@ -204,6 +212,9 @@ def compact_pages(caches, pool: PagePool, block_table):
     """Moves the held pages to the low end of the pool, in every layer of ``caches``, and rewrites counts and ``block_table`` (which must be the
     only one that names the pool's pages).  With L held pages the k-th held page at or above L moves to the k-th free page below L; the
     others stay.  Returns int32 [NUM_PAGES]: the new number of every held page, -1 for free ones."""
+    remap = _cabi.host().compact_pages(caches, pool.ref_counts, pool.page_size, block_table)
+    if remap is not None:
+        return remap
     B, max_blocks = _check_table(pool, block_table)
     groups, _ = _cache_tensors(caches, pool.num_pages, pool.page_size)
     device = _cabi.require_cuda(pool.ref_counts, block_table, *groups[0], *groups[1])
