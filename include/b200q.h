@@ -72,7 +72,7 @@ int b200q_device_status(int reset, void* stream);
  *   "attn.force_simple"  1 = always the one-warp-per-head attention kernel
  *   "peer.spin_limit", "tp.spin_limit"   flag probes after which b200q_peer_allgather / the wait of an exchange fused
  *                        into a kernel gives up and records event 5 (default 2^22; tests shorten it)
- *   "lora.cluster", "lora.span"     CTAs per cluster of b200q_lora_add (1, 2, 4, 8 or 16) and leading rows per cluster (default: by rows)
+ *   "lora.cluster"       CTAs per cluster of b200q_lora_add: 1, 2, 4, 8 or 16 (default: by rows)
  *   "no_pdl"             1 = launch without programmatic dependent launch */
 int b200q_set_tuning(const char* key, int value);
 
@@ -143,6 +143,13 @@ int b200q_gate_up_swiglu(int bits, const void* x, const uint8_t* gate_codes, con
  * previous kernel of the stream has ended when that is a kernel of this library: none of them writes to such arrays.
  * workspace: b200q_lora_workspace_bytes(rows, R) bytes of device scratch. */
 size_t b200q_lora_workspace_bytes(int64_t rows, int R);
+/* The adapters beside b200q_qmatvec: y[t] = cast(residual[t] + scaling[l] * B[l] (A[l] x[t]) + W x[t]), every sum in fp32 and one rounding
+ * (residual may be NULL).  Arguments as in b200q_qmatvec and b200q_lora_add; the matvec takes what b200q_scratch_next left for it. */
+size_t b200q_lora_qmatvec_workspace_bytes(int64_t rows, int64_t N, int R);
+int b200q_lora_qmatvec(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y,
+                       const void* a, const void* b, const float* scaling, const int32_t* ranks, const int32_t* ids, int rows, int64_t N,
+                       int64_t K, int group_size, int L, int R, int act_dtype, int scale_dtype, void* workspace, size_t workspace_bytes,
+                       void* stream);
 int b200q_lora_add(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
                    const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* workspace,
                    size_t workspace_bytes, void* stream);

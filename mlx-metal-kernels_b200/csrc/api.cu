@@ -89,6 +89,10 @@ int compact_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* 
                        size_t workspace_bytes, cudaStream_t stream);
 int lora_read_status(int reset, cudaStream_t stream);
 size_t lora_workspace_impl(int64_t rows, int R);
+size_t lora_qmatvec_workspace_impl(int64_t rows, int64_t N, int R);
+int lora_qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y,
+                      const void* a, const void* b, const float* scaling, const int32_t* ranks, const int32_t* ids, int rows, int64_t N, int64_t K,
+                      int group_size, int L, int R, int act_dtype, int scale_dtype, void* ws, size_t ws_bytes, cudaStream_t stream);
 int lora_add_impl(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
                   const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* ws, size_t ws_bytes,
                   cudaStream_t stream);
@@ -114,7 +118,7 @@ int wait_expiry_selftest_impl(uint32_t limit, uint32_t* probes_out, cudaStream_t
 int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros,
                  const void* residual, void* y, int B, int64_t N, int64_t K, int group_size, int act_dtype,
                  int scale_dtype, const void* residual_in, const void* norm_weight, int norm_w_dtype, float eps,
-                 void* z_out, void* normed_out, cudaStream_t stream);
+                 void* z_out, void* normed_out, cudaStream_t stream, const float* add32 = nullptr);
 int rope_kv_append_impl(const void* qkv, const float* cos_table, const float* sin_table, const int32_t* positions,
                         const int32_t* block_table, void* q_out, uint8_t* k_codes, uint8_t* v_codes, void* k_scales,
                         void* v_scales, int bits, int B, int Hq, int Hkv, int D, int page_size, int64_t num_pages,
@@ -457,6 +461,18 @@ int b200q_lora_add(const void* x, const void* y, void* out, const void* a, const
                    size_t workspace_bytes, void* stream) {
     tp_discard();
     return lora_add_impl(x, y, out, a, b, scaling, ranks, ids, rows, N, K, L, R, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+size_t b200q_lora_qmatvec_workspace_bytes(int64_t rows, int64_t N, int R) { return lora_qmatvec_workspace_impl(rows, N, R); }
+int b200q_lora_qmatvec(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y,
+                       const void* a, const void* b, const float* scaling, const int32_t* ranks, const int32_t* ids, int rows, int64_t N,
+                       int64_t K, int group_size, int L, int R, int act_dtype, int scale_dtype, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    tp_discard();
+    const int rc = lora_qmatvec_impl(bits, x, codes, scales, zeros, residual, y, a, b, scaling, ranks, ids, rows, N, K, group_size, L, R, act_dtype,
+                                     scale_dtype, workspace, workspace_bytes, (cudaStream_t)stream);
+    scratch_next(nullptr, 0);      // a call that ends early must not leave its scratch to the next one
+    return rc;
 }
 
 size_t b200q_reserve_pages_workspace_bytes(int B, int64_t num_pages) { return reserve_workspace_impl(B, num_pages); }

@@ -78,7 +78,8 @@ __global__ void __launch_bounds__(256) qgemv_generic_kernel(const __grid_constan
 #pragma unroll
         for (int m = 0; m < MATS; ++m) {
             const float s = warp_sum(acc[m]);
-            val[m] = round_act(fminf(fmaxf(s, -fmax_act), fmax_act), p.act_dtype);
+            const float c = fminf(fmaxf(s, -fmax_act), fmax_act);
+            val[m] = !GATE_UP && p.add32 != nullptr ? c : round_act(c, p.act_dtype);
         }
         if (lane == 0) {
             const int64_t o = (int64_t)b * p.N + row;
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(256) qgemv_generic_kernel(const __grid_constan
             } else {
                 float v = val[0];
                 if (p.residual != nullptr) v = load_as_f32(p.residual, p.act_dtype, o) + v;
+                else if (p.add32 != nullptr) v = p.add32[o] + v;
                 store(p.y, v);
             }
         }
@@ -221,6 +223,7 @@ GemvParams slice(const GemvParams& a, int b0, int bn) {
     p.x = in(a.x, a.K); p.res_in = in(a.res_in, a.K);
     p.z_out = out(a.z_out, a.K); p.normed_out = out(a.normed_out, a.K);
     p.residual = in(a.residual, a.N);
+    p.add32 = a.add32 ? a.add32 + (size_t)b0 * a.N : nullptr;
     p.y = out(a.y, a.N); p.gate_out = out(a.gate_out, a.N); p.up_out = out(a.up_out, a.N); p.act_out = out(a.act_out, a.N);
     p.B = bn;
     return p;
@@ -331,7 +334,7 @@ size_t norm_scratch_bytes_impl(int rows, int64_t K, int act_dtype) {
 int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros,
                  const void* residual, void* y, int B, int64_t N, int64_t K, int group_size, int act_dtype,
                  int scale_dtype, const void* residual_in, const void* norm_weight, int norm_w_dtype, float eps,
-                 void* z_out, void* normed_out, cudaStream_t stream) {
+                 void* z_out, void* normed_out, cudaStream_t stream, const float* add32) {
     const ScratchGuard guard;
     int tp_in_slot = -1, tp_out_slot = -1;
     tp_take(&tp_in_slot, &tp_out_slot);
@@ -349,7 +352,7 @@ int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scal
     p.x = x; p.res_in = residual_in; p.norm_w = norm_weight; p.eps = eps; p.norm_w_dtype = norm_w_dtype;
     p.z_out = z_out; p.normed_out = normed_out;
     p.w[0] = codes; p.s[0] = scales; p.z[0] = zeros;
-    p.residual = residual; p.y = y;
+    p.residual = residual; p.y = y; p.add32 = add32;
     p.B = B; p.N = (int)N; p.K = (int)K; p.G = group_size; p.Gn = (int)((K + group_size - 1) / group_size);
     p.act_dtype = act_dtype; p.scale_dtype = scale_dtype;
     p.row_bytes = bits == 4 ? (int)((K + 1) / 2) : (int)K;

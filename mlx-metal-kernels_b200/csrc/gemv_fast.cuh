@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(kThreads, kMinCtasPerSm) qgemv_kernel(const __
                         src[w * kTileRows * BC] = 0.0f;
                     }
                     if (need_row_pass && b < B) s *= xscale[b];
-                    val[m] = round_act(fminf(fmaxf(s, -fmax_act), fmax_act), p.act_dtype);
+                    const float c = fminf(fmaxf(s, -fmax_act), fmax_act);
+                    val[m] = !GATE_UP && p.add32 != nullptr ? c : round_act(c, p.act_dtype);
                 }
                 if (r < rows && b < B) {
                     const int64_t o = (int64_t)b * p.N + row0 + r;
@@ -373,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, kMinCtasPerSm) qgemv_kernel(const __
                     } else {
                         float v = val[0];
                         if (p.residual != nullptr) v = load_as_f32(p.residual, p.act_dtype, o) + v;
+                        else if (p.add32 != nullptr) v = p.add32[o] + v;
                         if (p.y != nullptr) store(p.y, v);
                         if (p.tp_out.world > 0) store_peers(v);
                     }

@@ -73,6 +73,7 @@ struct I8Params {
     const __half* s[2];
     const __half* z[2];
     const void* residual;
+    const float* add32;
     void* y;
     void* gate_out;
     void* up_out;
@@ -625,7 +626,8 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                 float sum = 0.0f;
 #pragma unroll 8
                 for (int i = 0; i < p.units; ++i) sum += src[(m * p.units + i) * (16 * NB)];
-                val[m] = i8_round_act(fminf(fmaxf(sum, -fmax_act), fmax_act), p.act_dtype);
+                const float c = fminf(fmaxf(sum, -fmax_act), fmax_act);
+                val[m] = p.add32 != nullptr ? c : i8_round_act(c, p.act_dtype);
             }
             const int row = r_lo + rb0 + rr;
             const int64_t o = (int64_t)b * p.N + row;
@@ -642,6 +644,8 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                 if (p.residual != nullptr) {
                     const uint16_t rb = res_smem ? resid[b * r_cnt + rb0 + rr] : reinterpret_cast<const uint16_t*>(p.residual)[o];
                     v = load_as_f32(&rb, p.act_dtype, 0) + v;
+                } else if (p.add32 != nullptr) {
+                    v = p.add32[o] + v;
                 }
                 if (p.y != nullptr) reinterpret_cast<unsigned short*>(p.y)[o] = bits_of(v);
             }
@@ -679,7 +683,7 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
         p.s[m] = (const __half*)q.s[m];
         p.z[m] = (const __half*)q.z[m];
     }
-    p.residual = q.residual; p.y = q.y; p.gate_out = q.gate_out; p.up_out = q.up_out; p.act_out = q.act_out;
+    p.residual = q.residual; p.add32 = q.add32; p.y = q.y; p.gate_out = q.gate_out; p.up_out = q.up_out; p.act_out = q.act_out;
     p.eps = q.eps; p.B = q.B; p.N = q.N; p.K = q.K; p.Gn = q.Gn; p.act_dtype = q.act_dtype; p.norm_w_dtype = q.norm_w_dtype;
     p.row_bytes = q.row_bytes; p.tp_out = q.tp_out; p.tp_in = q.tp_in;
     p.units = (p.row_bytes + kI8UnitBytes - 1) / kI8UnitBytes;

@@ -44,6 +44,7 @@ struct GemvParams {
     const void* z[2];
     // outputs
     const void* residual;   // plain: out = cast(residual + cast(y)); may be null
+    const float* add32;     // plain, instead of a residual: out = cast(add32 + y), [B, N]; may be null
     void* y;
     void* gate_out;
     void* up_out;

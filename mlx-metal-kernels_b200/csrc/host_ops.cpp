@@ -55,9 +55,9 @@ int (*p_head_rope)(const void*, const void*, void*, void*, const int64_t*, const
 int (*p_append)(const void*, int64_t, const float*, const float*, int64_t, int, int, const int32_t*, const int32_t*, const int32_t*, int, int,
                 const void*, const void*, int, float, void*, int, void*, void*, void*, void*, int64_t, int, int, int, int, int64_t, int, int,
                 void*) = nullptr;
-size_t (*p_lora_ws)(int64_t, int) = nullptr;
-int (*p_lora)(const void*, const void*, void*, const void*, const void*, const float*, const int32_t*, const int32_t*, int64_t, int64_t, int64_t,
-              int, int, int, void*, size_t, void*) = nullptr;
+size_t (*p_lora_ws)(int64_t, int64_t, int) = nullptr;
+int (*p_lora)(int, const void*, const uint8_t*, const void*, const void*, const void*, void*, const void*, const void*, const float*, const int32_t*,
+              const int32_t*, int, int64_t, int64_t, int, int, int, int, int, void*, size_t, void*) = nullptr;
 size_t (*p_reserve_ws)(int, int64_t) = nullptr;
 size_t (*p_copy_ws)(int, int64_t) = nullptr;
 size_t (*p_fork_ws)(int, int) = nullptr;
@@ -570,20 +570,17 @@ PyObject* lora_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (lr != nullptr && (!on(*lr, dev) || lr->scalar_type() != at::kInt || lr->dim() != 1 || lr->size(0) != L)) return none();
     const int act = dtype_code(x->scalar_type());
     void* st = stream_of(dev);
-    // one scratch block: the adapters' rows [rows, N], and what the two calls ask for
-    const int64_t low_bytes = (rows * m.n * 2 + 255) / 256 * 256;
-    const size_t lora_bytes = p_lora_ws(rows, (int)R), mat_bytes = p_scratch_bytes((int)rows, K, act), more = std::max(lora_bytes, mat_bytes);
-    Tensor scratch = empty({low_bytes + (int64_t)more}, at::kByte, dev);
+    // one scratch block for the adapters' rows and for the matvec
+    const size_t lora_bytes = (p_lora_ws(rows, m.n, (int)R) + 255) / 256 * 256, mat_bytes = p_scratch_bytes((int)rows, K, act);
+    Tensor scratch = empty({(int64_t)(lora_bytes + mat_bytes)}, at::kByte, dev);
     uint8_t* low = static_cast<uint8_t*>(scratch.mutable_data_ptr());
     std::vector<int64_t> shape(x->sizes().begin(), x->sizes().end());
     shape.back() = m.n;
     Tensor y = empty(shape, x->scalar_type(), dev);
-    if (p_lora(x->const_data_ptr(), ptr(res), low, la->const_data_ptr(), lb->const_data_ptr(), ls == nullptr ? nullptr : f32(ls), i32(lr), i32(ids),
-               rows, m.n, K, (int)L, (int)R, act, low + low_bytes, more, st) != 0)
-        return none();
-    p_scratch_next(mat_bytes ? low + low_bytes : nullptr, mat_bytes);
-    const int rc = p_qmatvec((int)bits, x->const_data_ptr(), codes(m.w), ptr(m.s), ptr(m.z), low, y.mutable_data_ptr(), (int)rows, m.n, K, (int)group,
-                             act, dtype_code(m.s->scalar_type()), st);
+    p_scratch_next(mat_bytes ? low + lora_bytes : nullptr, mat_bytes);      // the call below takes it, always
+    const int rc = p_lora((int)bits, x->const_data_ptr(), codes(m.w), ptr(m.s), ptr(m.z), ptr(res), y.mutable_data_ptr(), la->const_data_ptr(),
+                          lb->const_data_ptr(), ls == nullptr ? nullptr : f32(ls), i32(lr), i32(ids), (int)rows, m.n, K, (int)group, (int)L, (int)R, act,
+                          dtype_code(m.s->scalar_type()), low, lora_bytes, st);
     return rc == 0 ? THPVariable_Wrap(std::move(y)) : none();
 }
 
@@ -752,7 +749,7 @@ PyObject* bind(PyObject*, PyObject* table) {
         {"b200q_paged_gqa_decode", (void**)&p_attn}, {"b200q_paged_gqa_decode_window", (void**)&p_attn_window},
         {"b200q_paged_fp16_gqa_workspace_bytes", (void**)&p_plain_ws}, {"b200q_paged_fp16_gqa_decode", (void**)&p_plain_attn},
         {"b200q_paged_fp16_gqa_decode_checked", (void**)&p_plain_checked},
-        {"b200q_lora_workspace_bytes", (void**)&p_lora_ws}, {"b200q_lora_add", (void**)&p_lora},
+        {"b200q_lora_qmatvec_workspace_bytes", (void**)&p_lora_ws}, {"b200q_lora_qmatvec", (void**)&p_lora},
         {"b200q_reserve_pages_workspace_bytes", (void**)&p_reserve_ws}, {"b200q_copy_pages_workspace_bytes", (void**)&p_copy_ws},
         {"b200q_fork_sequences_workspace_bytes", (void**)&p_fork_ws}, {"b200q_compact_pages_workspace_bytes", (void**)&p_compact_ws},
         {"b200q_reserve_pages", (void**)&p_reserve}, {"b200q_release_sequences", (void**)&p_release},

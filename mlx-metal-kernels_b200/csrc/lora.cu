@@ -6,9 +6,8 @@
 // [rows, N] (out may be y).  Products are summed in fp32, the R values between the factors stay in fp32 (or in as many bits), and the
 // sum with y is rounded once.
 //
-// One launch for both products: a thread-block cluster per adapter and up to 16 of the rows that use it.  Rows are looked at in windows of 256;
-// of the rows of an adapter in a window every sixteenth leads a group (its cluster works, the others' end at once).  The CTAs of a
-// cluster cut K: every warp multiplies its pieces of the rows with the factor A on mma.sync, straight from global memory - the
+// One launch for both products: a thread-block cluster per adapter and up to 16 of the rows that use it.  Rows are looked at in windows of 256,
+// in which every CTA finds the groups; the clusters of a window take them in turn.  The CTAs of a cluster cut K: every warp multiplies its pieces of the rows with the factor A on mma.sync, straight from global memory - the
 // order of the summands is free, so a lane takes 16 contiguous bytes of a row as the k indices of two instructions.  The partial sums
 // meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp and round, a
 // lane with contiguous bytes of B again and 16 bytes of y, the next round's loads in flight during this one's products.  The values
@@ -25,12 +24,17 @@ namespace b200q {
 
 B200Q_DEFINE_STATUS_WORD(lora_read_status)
 
+int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros,
+                 const void* residual, void* y, int B, int64_t N, int64_t K, int group_size, int act_dtype,
+                 int scale_dtype, const void* residual_in, const void* norm_weight, int norm_w_dtype, float eps,
+                 void* z_out, void* normed_out, cudaStream_t stream, const float* add32);
+
 namespace {
 
 struct LoraParams {
     const void* x;            // [rows, K]
     const void* y;            // [rows, N] or null: 0
-    void* out;                // [rows, N]
+    void* out;                // [rows, N], in the rows' type or (out32) fp32
     const void* a;            // [L, R, K]
     const void* b;            // [L, N, R]
     const float* scaling;     // [L] or null: 1
@@ -38,7 +42,7 @@ struct LoraParams {
     const int32_t* ids;       // [rows]
     float* low;               // [rows, R] scratch of the general kernels
     int64_t rows, K, N;
-    int L, R;
+    int L, R, out32;
 };
 
 // Adapter of a row, or -1.
@@ -83,7 +87,8 @@ template <typename T> __global__ void __launch_bounds__(256) lora_expand_any_ker
             for (int r = 0; r < rank; ++r) s = fmaf(to_f32(b[r]), low[r], s);
             if (p.scaling) s *= p.scaling[id];
         }
-        reinterpret_cast<T*>(p.out)[it] = id < 0 ? y : from_f32<T>(to_f32(y) + s);
+        if (p.out32) reinterpret_cast<float*>(p.out)[it] = id < 0 ? to_f32(y) : to_f32(y) + s;
+        else reinterpret_cast<T*>(p.out)[it] = id < 0 ? y : from_f32<T>(to_f32(y) + s);
     }
 }
 
@@ -179,13 +184,16 @@ template <int STEPS, typename PIECE> struct Strip {
 
 // NT: rank tiles of 8 that a warp accumulates at a time.  NT 2 takes ranks by 16 (8 bytes of B per lane), NT 4 and 8 by 32 (16 bytes).
 template <typename T, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_kernel(const __grid_constant__ LoraParams p, int span, int vector_rows) {
+__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_kernel(const __grid_constant__ LoraParams p, int per_window, int vector_rows) {
     using Piece = std::conditional_t<NT <= 2, uint2, uint4>;
     constexpr int kPer = sizeof(Piece) / 2;                  // ranks in a lane's piece
     constexpr int kStep = 4 * kPer, kSteps = NT <= 4 ? 1 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float row_scale[kRows];
-    __shared__ unsigned match[kWindow / 32];
+    __shared__ __align__(16) int id_of[kWindow];             // -1: none, -2: no such row
+    __shared__ int before_of[kWindow];                       // rows of the same adapter ahead of a row in the window
+    __shared__ int leaders[kWindow];
+    __shared__ int leads[kWarps];
     __shared__ int row_of[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t cta = cluster_rank(), ctas = cluster_size();
@@ -195,41 +203,44 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
     T* hi = reinterpret_cast<T*>(smem + at.hi);
     T* lo = reinterpret_cast<T*>(smem + at.lo);
     const T* y = reinterpret_cast<const T*>(p.y);
-    T* out = reinterpret_cast<T*>(p.out);
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
     const int64_t chunks = (p.K + 31) / 32, per = (chunks + ctas - 1) / ctas;
     const int64_t c_lo = min(chunks, cta * per), c_hi = min(chunks, c_lo + per);
     const int64_t strips = (p.N + 31) / 32;
     pdl_launch_dependents();
-    bool waited = false;
 
-    const int64_t first = (int64_t)(blockIdx.x / ctas) * span;
-    for (int64_t lead = first; lead < min(p.rows, first + span); ++lead) {
-        // ---- the group that this row leads.  ids, ranks and factors belong to no kernel that may still run (see the header): they are
-        //      read before the wait ----
-        const int64_t row0 = lead / kWindow * kWindow;
-        const int id = max(adapter_of(p, lead), -1);
-        const bool same = row0 + threadIdx.x < p.rows && max(adapter_of(p, row0 + threadIdx.x), -1) == id;
-        const unsigned vote = __ballot_sync(0xFFFFFFFFu, same);
-        if (lane == 0) match[warp] = vote;
-        __syncthreads();
-        const int me = (int)(lead - row0);
-        int before = 0, mine = 0;                            // rows of the adapter ahead of the leader, and ahead of this thread's row
+    // ---- the window's groups: every sixteenth row of an adapter leads one.  ids, ranks and factors belong to no kernel that may
+    //      still run (see the header): they are read before the wait ----
+    const int64_t cluster = blockIdx.x / ctas, row0 = cluster / per_window * kWindow;
+    const int turn = (int)(cluster % per_window);
+    const int my_id = row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2;
+    id_of[threadIdx.x] = my_id;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < (int)threadIdx.x / 4; ++i) {
+        const int4 v = reinterpret_cast<const int4*>(id_of)[i];
+        before += (v.x == my_id) + (v.y == my_id) + (v.z == my_id) + (v.w == my_id);
+    }
+    for (int i = threadIdx.x / 4 * 4; i < (int)threadIdx.x; ++i) before += id_of[i] == my_id;
+    before_of[threadIdx.x] = before;
+    const unsigned lead_vote = __ballot_sync(0xFFFFFFFFu, my_id > -2 && before % kRows == 0);
+    if (lane == 0) leads[warp] = __popc(lead_vote);
+    __syncthreads();
+    int groups = 0, my_place = __popc(lead_vote & ((1u << lane) - 1u));
 #pragma unroll
-        for (int i = 0; i < kWindow / 32; ++i) {
-            const int c = __popc(match[i]);
-            if (i < me / 32) before += c;
-            if (i < warp) mine += c;
-        }
-        before += __popc(match[me / 32] & ((1u << (me & 31)) - 1u));
-        mine += __popc(vote & ((1u << lane) - 1u));
+    for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) my_place += leads[i];
+        groups += leads[i];
+    }
+    if (lead_vote >> lane & 1u) leaders[my_place] = threadIdx.x;
+    __syncthreads();
+
+    bool waited = false;
+    for (int turn_at = turn; turn_at < groups; turn_at += per_window) {      // all CTAs of a cluster agree
+        const int lead = leaders[turn_at], id = id_of[lead], ahead = before_of[lead];
         if (threadIdx.x < kRows) row_of[threadIdx.x] = -1;
-        if (before % kRows != 0) {                           // all CTAs of the cluster agree
-            __syncthreads();
-            continue;
-        }
         __syncthreads();
-        if (same && mine >= before && mine < before + kRows) row_of[mine - before] = threadIdx.x;
+        if (my_id == id && before >= ahead && before < ahead + kRows) row_of[before - ahead] = threadIdx.x;
         const int rank = id < 0 ? 0 : rank_of(p, id);
         const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
         const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
@@ -422,10 +433,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
                 if (t < 0 || n >= p.N) continue;
                 const float f = row_scale[g + 8 * half];
                 const T* e = reinterpret_cast<const T*>(&strip.y[half]);
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = id < 0 ? to_f32(e[i]) : fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e[i]));
+                const int64_t to = (row0 + t) * p.N + n;
+                if (p.out32) {
+                    float* dst = reinterpret_cast<float*>(p.out) + to;
+                    if (vector_rows) {
+                        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (n + i < p.N) dst[i] = v[i];
+                    }
+                    continue;
+                }
                 T o[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = id < 0 ? e[i] : from_f32<T>(fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e[i])));
-                T* dst = out + (row0 + t) * p.N + n;
+                for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
+                T* dst = reinterpret_cast<T*>(p.out) + to;
                 if (vector_rows) {
                     *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
                 } else {
@@ -443,18 +470,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
 }
 
 template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
+    const bool narrow = p.R <= 16 || p.R % 8 != 0 || ((uintptr_t)p.b & 15u) != 0, wide = !narrow && p.R > 32;
+    const int64_t windows = (p.rows + kWindow - 1) / kWindow, slots = (int64_t)sm_count() * (wide ? 1 : 2);
+    // CTAs per cluster: as many as leave every row a cluster of its own on the GPU at once, four at least - there are hardly as many
+    // adapters as rows - but fewer when the groups of 16 rows alone fill it
     int ctas = tuning_get("lora.cluster");
-    if (ctas <= 0) ctas = 8;
-    // leading rows per cluster: one, until the clusters of all rows are several times what the GPU holds
-    int64_t span = tuning_get("lora.span");
-    if (span <= 0) span = std::max<int64_t>(1, p.rows * ctas / ((int64_t)sm_count() * 8));
-    const int64_t clusters = (p.rows + span - 1) / span;
-    if (clusters > INT32_MAX / ctas || span > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
+    if (ctas <= 0) {
+        ctas = 16;
+        while (ctas > 4 && p.rows * ctas > sm_count()) ctas /= 2;
+        while (ctas > 1 && (p.rows + kRows - 1) / kRows * ctas > slots) ctas /= 2;
+    }
+    // clusters per window: one for each of its rows, as far as the GPU holds them
+    const int64_t rows = std::min<int64_t>(p.rows, kWindow), per_window = std::min(rows, std::max<int64_t>(1, slots / ctas / windows));
+    const int64_t clusters = windows * per_window;
+    if (clusters > INT32_MAX / ctas) return B200Q_ERR_UNSUPPORTED;
     const size_t smem = lora_smem(p.R).bytes;
-    void (*kernel)(const LoraParams, int, int) = p.R <= 16 || p.R % 8 != 0 || ((uintptr_t)p.b & 15u) != 0 ? lora_cluster_kernel<T, 2>
-                                               : p.R <= 32                                               ? lora_cluster_kernel<T, 4>
-                                                                                                         : lora_cluster_kernel<T, 8>;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    void (*kernel)(const LoraParams, int, int) = narrow ? lora_cluster_kernel<T, 2> : wide ? lora_cluster_kernel<T, 8> : lora_cluster_kernel<T, 4>;
+    if (smem > 40 * 1024 &&      // with the static part beyond what needs no asking
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
     if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return B200Q_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * ctas));
@@ -469,8 +502,8 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = tuning_get("no_pdl") ? 1 : 2;
-    const int vector_rows = p.N % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) & 15u) == 0;
-    return cudaLaunchKernelEx(&cfg, kernel, p, (int)span, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
+    const int vector_rows = p.N % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) & 15u) == 0;      // results in 16-byte pieces
+    return cudaLaunchKernelEx(&cfg, kernel, p, (int)per_window, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
 }
 bool cluster_takes(const LoraParams& p) {
     return p.K % 8 == 0 && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;
@@ -480,15 +513,40 @@ bool cluster_takes(const LoraParams& p) {
 
 size_t lora_workspace_impl(int64_t rows, int R) { return rows <= 0 || R <= 0 ? 0 : 4 * (size_t)rows * (size_t)R; }
 
+int lora_rows(const LoraParams& p, int dtype, size_t ws_bytes, cudaStream_t stream) {
+    if (cluster_takes(p)) return dtype == B200Q_F16 ? cluster_form<__half>(p, stream) : cluster_form<__nv_bfloat16>(p, stream);
+    if (p.low == nullptr || ws_bytes < lora_workspace_impl(p.rows, p.R)) return B200Q_ERR_WORKSPACE;
+    return dtype == B200Q_F16 ? any_size<__half>(p, stream) : any_size<__nv_bfloat16>(p, stream);
+}
+
 int lora_add_impl(const void* x, const void* y, void* out, const void* a, const void* b, const float* scaling, const int32_t* ranks,
                   const int32_t* ids, int64_t rows, int64_t N, int64_t K, int L, int R, int dtype, void* ws, size_t ws_bytes,
                   cudaStream_t stream) {
     if (x == nullptr || out == nullptr || a == nullptr || b == nullptr || ids == nullptr) return B200Q_ERR_BAD_ARG;
     if (rows <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0 || !is_act_dtype(dtype)) return B200Q_ERR_BAD_ARG;
     if (ws == nullptr || ws_bytes < lora_workspace_impl(rows, R)) return B200Q_ERR_WORKSPACE;
-    const LoraParams p = {x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R};
-    if (cluster_takes(p)) return dtype == B200Q_F16 ? cluster_form<__half>(p, stream) : cluster_form<__nv_bfloat16>(p, stream);
-    return dtype == B200Q_F16 ? any_size<__half>(p, stream) : any_size<__nv_bfloat16>(p, stream);
+    return lora_rows({x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R, 0}, dtype, ws_bytes, stream);
+}
+
+// The adapters' rows in fp32, then the matvec that adds them before its one rounding.
+static size_t low_rows_bytes(int64_t rows, int64_t N) { return (4 * (size_t)rows * (size_t)N + 255) / 256 * 256; }
+size_t lora_qmatvec_workspace_impl(int64_t rows, int64_t N, int R) {
+    return rows <= 0 || N <= 0 || R <= 0 ? 0 : low_rows_bytes(rows, N) + lora_workspace_impl(rows, R);
+}
+int lora_qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y,
+                      const void* a, const void* b, const float* scaling, const int32_t* ranks, const int32_t* ids, int rows, int64_t N, int64_t K,
+                      int group_size, int L, int R, int act_dtype, int scale_dtype, void* ws, size_t ws_bytes, cudaStream_t stream) {
+    if (x == nullptr || codes == nullptr || scales == nullptr || y == nullptr || a == nullptr || b == nullptr || ids == nullptr) return B200Q_ERR_BAD_ARG;
+    if ((bits != 4 && bits != 8) || rows <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0 || group_size <= 0 || !is_act_dtype(act_dtype) ||
+        !is_scale_dtype(scale_dtype))
+        return B200Q_ERR_BAD_ARG;
+    if (N > INT32_MAX || K > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
+    if (ws == nullptr || ws_bytes < lora_qmatvec_workspace_impl(rows, N, R)) return B200Q_ERR_WORKSPACE;
+    const size_t low = low_rows_bytes(rows, N);
+    const int rc = lora_rows({x, residual, ws, a, b, scaling, ranks, ids, (float*)((uint8_t*)ws + low), rows, K, N, L, R, 1}, act_dtype, ws_bytes - low, stream);
+    if (rc != B200Q_OK) return rc;
+    return qmatvec_impl(bits, x, codes, scales, zeros, nullptr, y, rows, N, K, group_size, act_dtype, scale_dtype, nullptr, nullptr, B200Q_F16, 0.0f,
+                        nullptr, nullptr, stream, (const float*)ws);
 }
 
 }  // namespace b200q

@@ -78,6 +78,7 @@ struct alignas(64) TsParams {
     const uint16_t* z[2];
     const float* col_scale;     // [B] factor of the result columns (rows that were scaled into fp16), or null
     const uint16_t* residual;   // plain: out = cast(residual + cast(y)); may be null
+    const float* add32;         // plain, instead: out = cast(add32 + y); may be null
     uint16_t* y;
     uint16_t* gate_out;
     uint16_t* up_out;
@@ -305,16 +306,18 @@ __device__ __forceinline__ float ts_float(bool bf, uint16_t u) {
 // The residual values of output row n for 4 columns, fetched ahead of the accumulators and before the first store (y may
 // alias the residual rows as far as the compiler knows).
 template <int MATS>
-__device__ __forceinline__ void ts_load_residual(const TsParams& p, int n, int b0, int nb, uint16_t (&res)[4]) {
+__device__ __forceinline__ void ts_load_residual(const TsParams& p, int n, int b0, int nb, uint32_t (&res)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         res[j] = 0;
-        if (MATS == 1 && p.residual != nullptr && n < p.N && j < nb) res[j] = p.residual[(size_t)(b0 + j) * p.N + n];
+        if (MATS != 1 || n >= p.N || j >= nb) continue;
+        if (p.residual != nullptr) res[j] = p.residual[(size_t)(b0 + j) * p.N + n];
+        else if (p.add32 != nullptr) res[j] = __float_as_uint(p.add32[(size_t)(b0 + j) * p.N + n]);
     }
 }
 // The epilogue of 4 columns (b0 .. b0 + nb of the batch): clamp, round, residual add or SwiGLU, store.
 template <int MATS, bool SPLIT>
-__device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&acc)[2][4], int n, int b0, int nb, const uint16_t (&res)[4]) {
+__device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&acc)[2][4], int n, int b0, int nb, const uint32_t (&res)[4]) {
     const bool bf = SPLIT && p.bf16;
     const float fmax_act = bf ? 3.3895313892515355e38f : 65504.0f;
 #pragma unroll
@@ -324,8 +327,13 @@ __device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&a
         const size_t o = (size_t)b * p.N + n;
         const float cs = SPLIT && p.col_scale != nullptr ? p.col_scale[b] : 1.0f;
         if (MATS == 1) {
-            float v = ts_round(bf, fminf(fmaxf((acc[0][j] + acc[1][j]) * cs, -fmax_act), fmax_act));
-            if (p.residual != nullptr) v = ts_float(bf, res[j]) + v;
+            float v = fminf(fmaxf((acc[0][j] + acc[1][j]) * cs, -fmax_act), fmax_act);
+            if (p.add32 != nullptr) {
+                v = __uint_as_float(res[j]) + v;
+            } else {
+                v = ts_round(bf, v);
+                if (p.residual != nullptr) v = ts_float(bf, (uint16_t)res[j]) + v;
+            }
             p.y[o] = ts_bits(bf, v);
         } else {
             const float v0 = ts_round(bf, fminf(fmaxf(acc[0][j] * cs, -fmax_act), fmax_act));
@@ -704,7 +712,7 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
             if (p.split == 1) {
                 if (it == 0) pdl_wait();
                 const int n = n0 + r, c0 = col_of(it) + grp * 4;
-                uint16_t res[4];
+                uint32_t res[4];
                 ts_load_residual<MATS>(p, n, c0, p.B - c0, res);
                 wait_bar(d_full, (uint32_t)it & 1u, EV_GEMV_FULL_WAIT, ok);
                 tc_fence_after();
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
                 for (int cs = 0; cs < ncols; cs += 16) {
                     const int nb = p.B - c0 - cs;              // may be more than 4
                     if (nb <= 0) break;
-                    uint16_t next[4];
+                    uint32_t next[4];
                     ts_load_residual<MATS>(p, n, c0 + cs + 16, cs + 16 < ncols ? nb - 16 : 0, next);
                     float acc[2][4] = {};
                     tc_ld4(lane_addr + (uint32_t)(cs + grp * 4), acc[0]);
@@ -771,12 +779,12 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
             pdl_wait();
             const int n = row_of(0) + r;
             const float* red = reinterpret_cast<const float*>(sbase + (red_base - base));
-            uint16_t res[4];
+            uint32_t res[4];
             ts_load_residual<MATS>(p, n, c0 + grp * 4, bcols - grp * 4, res);
             if (fast) wait_bar_cluster(red_bar, 0u, ok ? kTsWaitLimit : 64u);
 #pragma unroll 1
             for (int cs = grp * 4; cs < bcols; cs += 16) {
-                uint16_t next[4];
+                uint32_t next[4];
                 ts_load_residual<MATS>(p, n, c0 + cs + 16, bcols - cs - 16, next);
                 float acc[2][4] = {};
                 tc_ld4(lane_addr + (uint32_t)cs, acc[0]);
@@ -1051,7 +1059,7 @@ int qgemm_ts(int bits, const GemvParams& g, bool gate_up, cudaStream_t stream) {
             !tensor_map_2d(g.z[m], (uint64_t)g.Gn * 2, (uint64_t)g.N, kMetaGroups * 2, kRows, CU_TENSOR_MAP_SWIZZLE_32B, &p.zmap[m]))
             return B200Q_ERR_UNSUPPORTED;
     }
-    p.residual = (const uint16_t*)g.residual; p.y = (uint16_t*)g.y; p.gate_out = (uint16_t*)g.gate_out; p.up_out = (uint16_t*)g.up_out;
+    p.residual = (const uint16_t*)g.residual; p.add32 = g.add32; p.y = (uint16_t*)g.y; p.gate_out = (uint16_t*)g.gate_out; p.up_out = (uint16_t*)g.up_out;
     p.act_out = (uint16_t*)g.act_out;
     p.x = g.x;
     // Weights in two terms where the kernel that these calls had before, fp16 mma.sync with up to 16 rows a launch, takes codes and scales

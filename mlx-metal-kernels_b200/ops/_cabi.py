@@ -56,6 +56,9 @@ SIGNATURES = {
     "b200q_fork_sequences": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
     "b200q_compact_pages": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "b200q_lora_workspace_bytes": (_sz, [_i64, _i]),
+    "b200q_lora_qmatvec_workspace_bytes": (_sz, [_i64, _i64, _i]),
+    "b200q_lora_qmatvec": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i, _i, _i, _i, _i, _vp, _sz,
+                                _vp]),
     "b200q_lora_add": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "b200q_attention_stage_launches": (_i, [_i, _i, _i]),
     "b200q_attention_launches": (_i, [_i, _i, _i, _i]),

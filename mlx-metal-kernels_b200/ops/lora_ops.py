@@ -14,7 +14,7 @@ import torch
 
 from . import _cabi
 from .mlp_block_ops import _normalize_hidden_input, _restore_hidden_output, _validate_quantized_linear_shapes
-from .quant_ops import _resolve_matvec_backend, matvec_rows
+from .quant_ops import _resolve_matvec_backend
 from .rope_ops import int32_index
 
 
@@ -56,16 +56,15 @@ def _check(x2d, adapters, adapter_ids, lead, out_dim):
     return int32_index(adapter_ids.reshape(math.prod(lead)), "adapter_ids")
 
 
-def _launch(x2d, y2d, out2d, adapters, ids, device):
-    rows, K = x2d.shape
-    L, R, _ = adapters.a.shape
+def _factors(adapters):
+    """(tensors the kernels read - to be kept until the launch -, their addresses and sizes as the C calls take them)"""
     a, b = _cabi.contiguous(adapters.a), _cabi.contiguous(adapters.b)
     scaling, ranks = _cabi.contiguous(adapters.scaling), _cabi.contiguous(adapters.ranks)
-    lib = _cabi.load()
-    ws = torch.empty(max(16, lib.b200q_lora_workspace_bytes(rows, R)), dtype=torch.uint8, device=device)
-    _cabi.check(lib.b200q_lora_add(x2d.data_ptr(), _cabi.ptr(y2d), out2d.data_ptr(), a.data_ptr(), b.data_ptr(), _cabi.ptr(scaling),
-                                   _cabi.ptr(ranks), ids.data_ptr(), rows, b.shape[1], K, L, R, _cabi.dtype_code(x2d.dtype), ws.data_ptr(),
-                                   ws.numel(), _cabi.stream()), "b200q_lora_add")
+    return (a, b, scaling, ranks), (a.data_ptr(), b.data_ptr(), _cabi.ptr(scaling), _cabi.ptr(ranks)), (a.shape[0], a.shape[1])
+
+
+def _workspace(nbytes, device):
+    return torch.empty(max(16, nbytes), dtype=torch.uint8, device=device)
 
 
 def lora_add(y, x, adapters: LoraAdapters, adapter_ids):
@@ -81,15 +80,19 @@ def lora_add(y, x, adapters: LoraAdapters, adapter_ids):
     if out.numel() == 0:
         return out
     with _cabi.on_device(device):
-        _launch(_cabi.contiguous(x2d), _cabi.contiguous(y), out, adapters, ids, device)
+        x2d, y = _cabi.contiguous(x2d), _cabi.contiguous(y)
+        rows, K = x2d.shape
+        keep, factors, (L, R) = _factors(adapters)
+        lib = _cabi.load()
+        ws = _workspace(lib.b200q_lora_workspace_bytes(rows, R), device)
+        _cabi.check(lib.b200q_lora_add(x2d.data_ptr(), y.data_ptr(), out.data_ptr(), *factors, ids.data_ptr(), rows, y.shape[-1], K, L, R,
+                                       _cabi.dtype_code(x.dtype), ws.data_ptr(), ws.numel(), _cabi.stream()), "b200q_lora_add")
     return out
 
 
 def lora_quantized_linear(x, w, scales, zeros, adapters: LoraAdapters, adapter_ids, *, bits=4, group_size=32, residual=None, backend="auto"):
-    """``quantized_linear`` with the adapter of every row: [B,K] / [B,S,K] -> N features.  The adapters' part (with ``residual`` [.., N]: its
-    sum with that) is rounded to x.dtype and goes into the shared product as the residual row does in the MLP block:
-    y = cast(cast(residual + scaling * B (A x)) + cast(W x)).  In this order the product's weights are on their way while the adapters
-    are computed."""
+    """``quantized_linear`` with the adapter of every row: [B,K] / [B,S,K] -> N features, y = W x + scaling * B (A x), plus ``residual``
+    [.., N] where given.  All sums are fp32 and rounded once, at the end."""
     out = _cabi.host().lora_linear(bits, x, w, scales, zeros, group_size, backend, adapters, adapter_ids, residual)
     if out is not None:
         return out
@@ -103,10 +106,14 @@ def lora_quantized_linear(x, w, scales, zeros, adapters: LoraAdapters, adapter_i
     if x2d.shape[0] == 0:
         return torch.empty((*shape[:-1], out_dim), dtype=x.dtype, device=device)
     with _cabi.on_device(device):
-        x2d = _cabi.contiguous(x2d)
-        if residual is not None:
-            residual = _cabi.contiguous(residual.reshape(-1, out_dim).to(x.dtype))
-        low = torch.empty((x2d.shape[0], out_dim), dtype=x.dtype, device=device)
-        _launch(x2d, residual, low, adapters, ids, device)
-        y = matvec_rows(bits, x2d, w, scales, zeros, group_size, low)
+        x2d, w = _cabi.contiguous(x2d), _cabi.contiguous(w.to(torch.uint8))
+        scales, zeros = _cabi.scale_pair(scales, zeros)
+        residual = None if residual is None else _cabi.contiguous(residual.reshape(-1, out_dim).to(x.dtype))
+        rows, K = x2d.shape
+        keep, factors, (L, R) = _factors(adapters)
+        y = torch.empty((rows, out_dim), dtype=x.dtype, device=device)
+        ws = _workspace(_cabi.load().b200q_lora_qmatvec_workspace_bytes(rows, out_dim, R), device)
+        _cabi.call_with_scratch("b200q_lora_qmatvec", rows, K, x2d, bits, x2d.data_ptr(), w.data_ptr(), scales.data_ptr(), _cabi.ptr(zeros),
+                                _cabi.ptr(residual), y.data_ptr(), *factors, ids.data_ptr(), rows, out_dim, K, group_size, L, R,
+                                _cabi.dtype_code(x.dtype), _cabi.dtype_code(scales.dtype), ws.data_ptr(), ws.numel(), _cabi.stream())
     return _restore_hidden_output(y, shape)

@@ -83,3 +83,18 @@ def test_c_abi_refuses_bad_arguments():
         args[i] = v
         assert lib.b200q_lora_add(*args) == -4, (i, v)
     assert lib.b200q_lora_workspace_bytes(2, 4) == 32 and lib.b200q_lora_workspace_bytes(0, 4) == 0
+    good = [4, 16, 16, 16, 16, None, 16, 16, 16, None, None, 16, 2, 32, 64, 32, 3, 4, 0, 0, 16, 1 << 20, None]
+    for i, v in ((0, 5), (1, None), (2, None), (3, None), (6, None), (7, None), (8, None), (11, None), (12, 0), (13, 0), (14, 0), (15, 0), (16, 0),
+                 (17, 0), (18, 2), (19, 3)):
+        args = list(good)
+        args[i] = v
+        assert lib.b200q_lora_qmatvec(*args) == -1, (i, v)
+    for i, v in ((20, None), (21, 2 * 32 * 4)):
+        args = list(good)
+        args[i] = v
+        assert lib.b200q_lora_qmatvec(*args) == -4, (i, v)
+    for i in (13, 14):
+        args = list(good)
+        args[i] = 2 ** 31
+        assert lib.b200q_lora_qmatvec(*args) == -2
+    assert lib.b200q_lora_qmatvec_workspace_bytes(2, 32, 4) >= 2 * 32 * 4 + 32 and lib.b200q_lora_qmatvec_workspace_bytes(0, 32, 4) == 0
