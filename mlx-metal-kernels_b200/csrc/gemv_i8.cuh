@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
     float* red = reinterpret_cast<float*>(smem);                   // sums of squares of the norm prologue, one per 32 pieces
     float* part = reinterpret_cast<float*>(smem + p.off_part);     // [tiles of a batch][mats][units][16 rows][NB]
     uint16_t* resid = reinterpret_cast<uint16_t*>(smem + p.off_res);
+    float* add = reinterpret_cast<float*>(smem + p.off_res);
 
     const int rank = KS == 1 ? 0 : blockIdx.x % KS;
     const int cta = blockIdx.x / KS;
@@ -365,11 +366,13 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
         if ((int)threadIdx.x < p.tp_in.world && !tp_wait_source(p.tp_in, threadIdx.x)) atomicMax(&g_device_status, (int)EV_PEER_WAIT);
         __syncthreads();
     }
-    const bool res_smem = p.residual != nullptr && r_cnt * B <= kI8MaxRes;
+    const bool res_smem = (p.residual != nullptr || p.add32 != nullptr) && r_cnt * B <= kI8MaxRes;
     if (res_smem)
         for (int i = threadIdx.x; i < r_cnt * B; i += kI8Threads) {
             const int b = i / r_cnt;
-            resid[i] = reinterpret_cast<const uint16_t*>(p.residual)[(size_t)b * p.N + r_lo + (i - b * r_cnt)];
+            const size_t o = (size_t)b * p.N + r_lo + (i - b * r_cnt);
+            if (p.add32 != nullptr) add[i] = p.add32[o];
+            else resid[i] = reinterpret_cast<const uint16_t*>(p.residual)[o];
         }
     // Items: 8-value pieces of the padded rows.  A warp's 32 pieces lie in one row (a padded row is a multiple of 32 pieces).
     // The loop stays small on purpose: hoisting four loads per thread made every launch 0.4 us longer (instruction fetch)
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                     const uint16_t rb = res_smem ? resid[b * r_cnt + rb0 + rr] : reinterpret_cast<const uint16_t*>(p.residual)[o];
                     v = load_as_f32(&rb, p.act_dtype, 0) + v;
                 } else if (p.add32 != nullptr) {
-                    v = p.add32[o] + v;
+                    v = (res_smem ? add[b * r_cnt + rb0 + rr] : p.add32[o]) + v;
                 }
                 if (p.y != nullptr) reinterpret_cast<unsigned short*>(p.y)[o] = bits_of(v);
             }
@@ -713,7 +716,7 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
         p.off_zero = off;  off += S::XU + 128;
         p.off_xd = off;    off += i8_align((uint32_t)q.B * p.xstride, 128);
         p.off_cst = off;   off += (uint32_t)q.B * p.cstride;
-        p.off_res = off;   off += p.residual != nullptr ? i8_align((uint32_t)std::min(r_max * q.B, kI8MaxRes) * 2, 128) : 0;
+        p.off_res = off;   off += p.residual || p.add32 ? i8_align((uint32_t)std::min(r_max * q.B, kI8MaxRes) * (p.add32 ? 4 : 2), 128) : 0;
         off = i8_align(off, 128);
         p.off_part = off;  off += i8_align((uint32_t)(p.batch * tile_bytes), 128);
         p.off_meta = off;  off += kI8Warps * 2 * p.meta_slot;

@@ -112,8 +112,8 @@ template <typename T> int any_size(const LoraParams& p, cudaStream_t stream) {
 }
 
 // ---- the cluster kernel: K a multiple of 8, R a multiple of 4 up to 256, 16-byte aligned factors and rows ------------------------
-constexpr int kRows = 16, kWarps = 8, kMaxRank = 256, kRankBlock = 64, kMaxCtas = 16;
-constexpr int kWindow = kWarps * 32;      // rows that one group may come from: an id per thread
+constexpr int kRows = 16, kMaxRank = 256, kRankBlock = 64, kMaxCtas = 16;
+constexpr int kWindow = 256;              // rows that one group may come from
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -164,30 +164,24 @@ struct LoraSmem {
     int low_stride;           // 16-bit values per row of a term: the rank in whole steps of 32, and 8 against bank conflicts
     size_t part, cta, hi, lo, bytes;
 };
-__host__ __device__ inline LoraSmem lora_smem(int R) {
+__host__ __device__ inline LoraSmem lora_smem(int R, int warps) {
     LoraSmem s;
     const int block = R < kRankBlock ? (R + 7) / 8 * 8 : kRankBlock;
     s.low_stride = (R + 31) / 32 * 32 + 8;
     s.part = 0;
-    s.cta = s.part + sizeof(float) * kWarps * kRows * block;
+    s.cta = s.part + sizeof(float) * warps * kRows * block;
     s.hi = s.cta + sizeof(float) * kRows * ((R + 7) / 8 * 8);
     s.lo = s.hi + 2 * (size_t)kRows * s.low_stride;
     s.bytes = s.lo + 2 * (size_t)kRows * s.low_stride;
     return s;
 }
 
-// A round's part of B and of y, loaded ahead: STEPS pieces of B for each of its four tiles.
-template <int STEPS, typename PIECE> struct Strip {
-    PIECE w[STEPS][4];
-    uint4 y[2];
-};
-
 // NT: rank tiles of 8 that a warp accumulates at a time.  NT 2 takes ranks by 16 (8 bytes of B per lane), NT 4 and 8 by 32 (16 bytes).
-template <typename T, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_kernel(const __grid_constant__ LoraParams p, int per_window, int vector_rows) {
+template <typename T, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __grid_constant__ LoraParams p, int per_window, int vector_rows) {
     using Piece = std::conditional_t<NT <= 2, uint2, uint4>;
     constexpr int kPer = sizeof(Piece) / 2;                  // ranks in a lane's piece
-    constexpr int kStep = 4 * kPer, kSteps = NT <= 4 ? 1 : 2;
+    constexpr int kStep = 4 * kPer;                          // ranks of a round
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float row_scale[kRows];
     __shared__ __align__(16) int id_of[kWindow];             // -1: none, -2: no such row
@@ -197,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
     __shared__ int row_of[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t cta = cluster_rank(), ctas = cluster_size();
-    const LoraSmem at = lora_smem(p.R);
+    const LoraSmem at = lora_smem(p.R, kWarps);
     float* part = reinterpret_cast<float*>(smem + at.part);
     float* own = reinterpret_cast<float*>(smem + at.cta);
     T* hi = reinterpret_cast<T*>(smem + at.hi);
@@ -213,16 +207,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
     //      still run (see the header): they are read before the wait ----
     const int64_t cluster = blockIdx.x / ctas, row0 = cluster / per_window * kWindow;
     const int turn = (int)(cluster % per_window);
-    const int my_id = row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2;
-    id_of[threadIdx.x] = my_id;
+    const bool looks = kWarps * 32 <= kWindow || threadIdx.x < kWindow;
+    const int my_id = looks && row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2;
+    if (looks) id_of[threadIdx.x] = my_id;
     __syncthreads();
     int before = 0;
-    for (int i = 0; i < (int)threadIdx.x / 4; ++i) {
+    for (int i = 0; my_id > -2 && i < (int)threadIdx.x / 4; ++i) {
         const int4 v = reinterpret_cast<const int4*>(id_of)[i];
         before += (v.x == my_id) + (v.y == my_id) + (v.z == my_id) + (v.w == my_id);
     }
-    for (int i = threadIdx.x / 4 * 4; i < (int)threadIdx.x; ++i) before += id_of[i] == my_id;
-    before_of[threadIdx.x] = before;
+    for (int i = threadIdx.x / 4 * 4; my_id > -2 && i < (int)threadIdx.x; ++i) before += id_of[i] == my_id;
+    if (looks) before_of[threadIdx.x] = before;
     const unsigned lead_vote = __ballot_sync(0xFFFFFFFFu, my_id > -2 && before % kRows == 0);
     if (lane == 0) leads[warp] = __popc(lead_vote);
     __syncthreads();
@@ -271,42 +266,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
         const int t0 = row_of[g], t1 = row_of[g + 8];
         const bool r0 = t0 >= 0, r1 = t1 >= 0;
 
-        // a round's loads: instruction j's column n is 32 s + 8 (n / 2) + 2 j + n % 2, so that a lane's results are columns 32 s + 8 q .. + 7
-        // of rows g and g + 8
-        auto load_b = [&](Piece (&w)[kSteps][4], int64_t s, int k0) {
-            const int64_t col = s * 32 + (g >> 1) * 8 + (g & 1);
-#pragma unroll
-            for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k = k0 + st * kStep + q * kPer;
-                    Piece v = {};
-                    if (k < rank && col + 2 * j < p.N) v = __ldg(reinterpret_cast<const Piece*>(b + (col + 2 * j) * p.R + k));
-                    w[st][j] = v;
-                }
-        };
-        auto load_strip = [&](Strip<kSteps, Piece>& strip, int64_t s) {
-            load_b(strip.w, s, 0);
-            const int64_t n = s * 32 + q * 8;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int t = half ? t1 : t0;
-                strip.y[half] = zero;
-                if (y == nullptr || t < 0 || n >= p.N) continue;
-                const T* src = y + (row0 + t) * p.N + n;
-                if (vector_rows) {
-                    strip.y[half] = *reinterpret_cast<const uint4*>(src);
-                } else {
-                    T e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = n + i < p.N ? src[i] : from_f32<T>(0.0f);
-                    strip.y[half] = *reinterpret_cast<const uint4*>(e);
-                }
-            }
-        };
+        // a round's loads of B, a lane's piece for each of four instructions: j's column n is 32 s + 8 (n / 2) + 2 j + n % 2, so that a
+        // lane's results are columns 32 s + 8 q .. + 7 of rows g and g + 8
         const int64_t s_first = (int64_t)cta * kWarps + warp, s_step = (int64_t)ctas * kWarps;
-        Strip<kSteps, Piece> strip;
-        if (s_first < strips) load_strip(strip, s_first);
+        const int first_col = (g >> 1) * 8 + (g & 1), b_next = 2 * p.R;
+        const T* b_lane = b + (s_first * 32 + first_col) * p.R + q * kPer;
+        const bool ragged = rank % kPer != 0;
+        auto load_b = [&](Piece (&w)[4], const T* from, int64_t s, int k0) {
+            const int k = k0 + q * kPer;
+            const bool whole = s * 32 + 32 <= p.N;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = {};
+                if (k < rank && (whole || s * 32 + first_col + 2 * j < p.N)) w[j] = __ldg(reinterpret_cast<const Piece*>(from + j * b_next + k0));
+            }
+            if (ragged && k < rank && k + kPer > rank)       // values behind the rank are not the adapter's
+#pragma unroll
+                for (int j = 0; j < 4; ++j) keep_ranks(w[j], rank - k);
+        };
+        Piece w[4];
+        if (NT <= 4) load_b(w, b_lane, s_first, 0);          // NT 8 has no registers for it yet
 
         // ---- rows times A: the CTA's chunks of 32 k, dealt to its warps; a lane holds k = 8q .. 8q + 7 of a chunk ----
         const T* x0 = reinterpret_cast<const T*>(p.x) + (row0 + max(t0, 0)) * p.K + q * 8;
@@ -358,6 +337,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
         }
         // ---- the CTAs' sums meet in every CTA: a warp per row, as two terms and a power of two ----
         cluster_arrive();
+        if (NT > 4) load_b(w, b_lane, s_first, 0);
         cluster_wait();
         for (int r = warp; r < kRows; r += kWarps) {
             const bool used = row_of[r] >= 0;
@@ -395,47 +375,68 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
         __syncthreads();
 
         // ---- times B ----
-        for (int64_t s = s_first; s < strips; s += s_step) {
-            Strip<kSteps, Piece> next;
-            if (s + s_step < strips) load_strip(next, s + s_step);
+        float f[2];
+        f[0] = row_scale[g];
+        f[1] = row_scale[g + 8];
+        for (int64_t s = s_first; s < strips; s += s_step, b_lane += s_step * 32 * p.R) {
+            const int64_t n = s * 32 + q * 8;
+            uint4 was[2] = {zero, zero};                     // y of the lane's columns
+            if (y != nullptr)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int t = half ? t1 : t0;
+                    if (t < 0 || n >= p.N) continue;
+                    const T* src = y + (row0 + t) * p.N + n;
+                    if (vector_rows) {
+                        was[half] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        T e[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) e[i] = n + i < p.N ? src[i] : from_f32<T>(0.0f);
+                        was[half] = *reinterpret_cast<const uint4*>(e);
+                    }
+                }
             float acc[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-            auto multiply = [&](Piece (&w)[kSteps][4], int k0) {
-#pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    const int k = k0 + st * kStep + q * kPer;
-                    if (k0 + st * kStep >= rank) break;
+            int k0 = 0;
+            do {
+                Piece next[4];
+                if (k0 + kStep < rank) load_b(next, b_lane, s, k0 + kStep);
+                else if (s + s_step < strips) load_b(next, b_lane + s_step * 32 * p.R, s + s_step, 0);
+                if (k0 < rank) {
+                    const int k = k0 + q * kPer;
                     const Piece h0 = *reinterpret_cast<const Piece*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const Piece*>(hi + (g + 8) * at.low_stride + k);
                     const Piece l0 = *reinterpret_cast<const Piece*>(lo + g * at.low_stride + k), l1 = *reinterpret_cast<const Piece*>(lo + (g + 8) * at.low_stride + k);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        Piece v = w[st][j];
-                        if (k + kPer > rank) keep_ranks(v, rank - k);      // values behind the rank are not the adapter's
-                        mma16(acc[j], h0.x, h1.x, h0.y, h1.y, v.x, v.y, (const T*)nullptr);
-                        mma16(acc[j], l0.x, l1.x, l0.y, l1.y, v.x, v.y, (const T*)nullptr);
-                        if constexpr (kPer == 8) {
-                            mma16(acc[j], h0.z, h1.z, h0.w, h1.w, v.z, v.w, (const T*)nullptr);
-                            mma16(acc[j], l0.z, l1.z, l0.w, l1.w, v.z, v.w, (const T*)nullptr);
+                        mma16(acc[j], h0.x, h1.x, h0.y, h1.y, w[j].x, w[j].y, (const T*)nullptr);
+                        mma16(acc[j], l0.x, l1.x, l0.y, l1.y, w[j].x, w[j].y, (const T*)nullptr);
+                    }
+                    if constexpr (kPer == 8) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            mma16(acc[j], h0.z, h1.z, h0.w, h1.w, w[j].z, w[j].w, (const T*)nullptr);
+                            mma16(acc[j], l0.z, l1.z, l0.w, l1.w, w[j].z, w[j].w, (const T*)nullptr);
                         }
                     }
                 }
-            };
-            multiply(strip.w, 0);
-            for (int k0 = kSteps * kStep; k0 < rank; k0 += kSteps * kStep) {
-                load_b(strip.w, s, k0);
-                multiply(strip.w, k0);
-            }
-            const int64_t n = s * 32 + q * 8;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = next[j];
+                k0 += kStep;
+            } while (k0 < rank);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int t = half ? t1 : t0;
                 if (t < 0 || n >= p.N) continue;
-                const float f = row_scale[g + 8 * half];
-                const T* e = reinterpret_cast<const T*>(&strip.y[half]);
                 float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = id < 0 ? to_f32(e[i]) : fmaf(acc[i >> 1][2 * half + (i & 1)], f, to_f32(e[i]));
+                for (int i = 0; i < 8; ++i) v[i] = acc[i >> 1][2 * half + (i & 1)] * f[half];
+                if (y != nullptr) {
+                    const T* e = reinterpret_cast<const T*>(&was[half]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = id < 0 ? to_f32(e[i]) : v[i] + to_f32(e[i]);
+                }
                 const int64_t to = (row0 + t) * p.N + n;
                 if (p.out32) {
                     float* dst = reinterpret_cast<float*>(p.out) + to;
@@ -447,21 +448,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
                         for (int i = 0; i < 8; ++i)
                             if (n + i < p.N) dst[i] = v[i];
                     }
-                    continue;
-                }
-                T o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
-                T* dst = reinterpret_cast<T*>(p.out) + to;
-                if (vector_rows) {
-                    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
                 } else {
+                    T o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (n + i < p.N) dst[i] = o[i];
+                    for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
+                    T* dst = reinterpret_cast<T*>(p.out) + to;
+                    if (vector_rows) {
+                        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (n + i < p.N) dst[i] = o[i];
+                    }
                 }
             }
-            strip = next;
         }
         cluster_wait();                                      // also: no CTA overwrites its sums for the next row while another reads them
         __syncthreads();
@@ -471,27 +471,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1) lora_cluster_ker
 
 template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
     const bool narrow = p.R <= 16 || p.R % 8 != 0 || ((uintptr_t)p.b & 15u) != 0, wide = !narrow && p.R > 32;
-    const int64_t windows = (p.rows + kWindow - 1) / kWindow, slots = (int64_t)sm_count() * (wide ? 1 : 2);
-    // CTAs per cluster: as many as leave every row a cluster of its own on the GPU at once, four at least - there are hardly as many
-    // adapters as rows - but fewer when the groups of 16 rows alone fill it
+    const int64_t windows = (p.rows + kWindow - 1) / kWindow, slots = (int64_t)sm_count() * 2;
+    // CTAs per cluster.  As many as leave every row a cluster of its own on the GPU at once; four at least, or eight where a group reads a MB
+    // of factors - there are hardly as many adapters as rows - but fewer when the groups of 16 rows alone fill the GPU.  With the
+    // projection, us for 4 / 8 / 16: one row, rank 16, 4096 x 4096: 12.3 / 10.5 / 9.9; 32 rows, rank 64, 6144 x 4096: 37.5 / 31.3 / 37.1; 128 rows of 32
+    // adapters, rank 16: 22.2 / 25.6 / 33.3; 512 rows, rank 64, 14336 x 4096: 127 / 120 / 132.
     int ctas = tuning_get("lora.cluster");
     if (ctas <= 0) {
+        const int least = (int64_t)p.R * (p.K + p.N) >= 512 * 1024 ? 8 : 4;
         ctas = 16;
-        while (ctas > 4 && p.rows * ctas > sm_count()) ctas /= 2;
+        while (ctas > least && p.rows * ctas > slots) ctas /= 2;
         while (ctas > 1 && (p.rows + kRows - 1) / kRows * ctas > slots) ctas /= 2;
     }
     // clusters per window: one for each of its rows, as far as the GPU holds them
     const int64_t rows = std::min<int64_t>(p.rows, kWindow), per_window = std::min(rows, std::max<int64_t>(1, slots / ctas / windows));
     const int64_t clusters = windows * per_window;
     if (clusters > INT32_MAX / ctas) return B200Q_ERR_UNSUPPORTED;
-    const size_t smem = lora_smem(p.R).bytes;
-    void (*kernel)(const LoraParams, int, int) = narrow ? lora_cluster_kernel<T, 2> : wide ? lora_cluster_kernel<T, 8> : lora_cluster_kernel<T, 4>;
+    const int warps = 8;
+    const size_t smem = lora_smem(p.R, warps).bytes;
+    void (*kernel)(const LoraParams, int, int) = narrow ? lora_cluster_kernel<T, 2, 8> : wide ? lora_cluster_kernel<T, 8, 8> : lora_cluster_kernel<T, 4, 8>;
     if (smem > 40 * 1024 &&      // with the static part beyond what needs no asking
          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
     if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return B200Q_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * ctas));
-    cfg.blockDim = dim3(kWarps * 32);
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
