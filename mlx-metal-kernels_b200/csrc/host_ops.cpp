@@ -494,32 +494,29 @@ PyObject* head_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return out;
 }
 
-// norm_rope_append(qkv, cos, sin, positions, sequences or None, block_table, n_heads, q_weight, k_weight, eps, layout, bits, k pages, v pages,
-//                  k scales or None, v scales or None, group_size, shape) -> q or None
-PyObject* norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    int64_t Hq, bits, group, dims[4];
-    if (p_append == nullptr || n_args != 18 || !as_int(a[6], &Hq) || !as_int(a[11], &bits) || !as_int(a[16], &group) || !PyTuple_Check(a[17]) ||
-        PyTuple_GET_SIZE(a[17]) != 4)
-        return none();
-    for (int i = 0; i < 4; ++i)
-        if (!as_int(PyTuple_GET_ITEM(a[17], i), &dims[i]) || dims[i] <= 0) return none();
+// What both append operators share, a: qkv, cos, sin, positions, n_heads, sequences or None, q_weight, k_weight, eps, layout; pages and
+// scales (null for plain pages) of the shape `dims`.
+PyObject* append_rows(PyObject* const* a, const Tensor* bt, const Tensor* kp, const Tensor* vp, const Tensor* ks, const Tensor* vs, const int64_t* dims,
+                      int64_t bits, int64_t group) {
+    int64_t Hq;
+    if (!as_int(a[4], &Hq)) return none();
     const int64_t pages = dims[0], P = dims[1], Hkv = dims[2], D = dims[3];
-    const Tensor *x = as_tensor(a[0]), *seq = as_tensor(a[4]), *bt = as_tensor(a[5]);
+    if (pages <= 0 || P <= 0 || Hkv <= 0 || D <= 0) return none();
+    const Tensor *x = as_tensor(a[0]), *seq = as_tensor(a[5]);
     const int dev = current_device_of(x);
-    if (dev < 0 || bt == nullptr || (seq == nullptr && a[4] != Py_None) || x->dim() != 2 || !act_dtype(x->scalar_type()) || Hq <= 0 ||
+    if (dev < 0 || bt == nullptr || (seq == nullptr && a[5] != Py_None) || x->dim() != 2 || !act_dtype(x->scalar_type()) || Hq <= 0 ||
         Hq > INT32_MAX || Hkv > INT32_MAX || P > INT32_MAX || x->size(0) <= 0 || x->size(1) != (Hq + 2 * Hkv) * D || x->stride(1) != 1 ||
         x->stride(0) < x->size(1))
         return none();
     const int64_t T = x->size(0);
     Rotation r;
-    if (!rotation(r, a[1], a[2], a[3], a[7], a[8], a[9], a[10], D, dev) || r.pos->dim() != 1 || r.pos->size(0) != T) return none();
+    if (!rotation(r, a[1], a[2], a[3], a[6], a[7], a[8], a[9], D, dev) || r.pos->dim() != 1 || r.pos->size(0) != T) return none();
     if (!on(*bt, dev) || bt->scalar_type() != at::kInt || bt->dim() != 2 || bt->size(0) <= 0 || bt->size(1) <= 0 || bt->size(0) > INT32_MAX ||
         bt->size(1) > INT32_MAX)
         return none();
     if (seq == nullptr ? T != bt->size(0) : !on(*seq, dev) || seq->scalar_type() != at::kInt || seq->dim() != 1 || seq->size(0) != T) return none();
     const bool plain = bits == 16;
     if (!plain && ((bits != 4 && bits != 8) || group <= 0 || group > INT32_MAX)) return none();
-    const Tensor *kp = as_tensor(a[12]), *vp = as_tensor(a[13]), *ks = as_tensor(a[14]), *vs = as_tensor(a[15]);
     const int64_t slots = pages * P * Hkv, width = bits == 4 ? (D + 1) / 2 : D;
     for (const Tensor* t : {kp, vp})
         if (t == nullptr || !on(*t, dev) || t->scalar_type() != (plain ? x->scalar_type() : at::kByte) || t->dim() != 4 || t->size(0) != pages ||
@@ -536,6 +533,30 @@ PyObject* norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                             out.mutable_data_ptr(), (int)bits, w(kp), w(vp), plain ? nullptr : w(ks), plain ? nullptr : w(vs), T, (int)Hq,
                             (int)Hkv, (int)D, (int)P, pages, plain ? 0 : (int)group, dtype_code(x->scalar_type()), stream_of(dev));
     return rc == 0 ? THPVariable_Wrap(std::move(out)) : none();
+}
+
+// norm_rope_append(qkv, cos, sin, positions, n_heads, sequences, q_weight, k_weight, eps, layout, cache) -> q or None: quantised pages
+PyObject* norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (p_append == nullptr || n_args != 11) return none();
+    Attr bits_o(a[10], s_bits), group_o(a[10], s_group_size), shape(a[10], s_shape), kq(a[10], s_kq), vq(a[10], s_vq), ks(a[10], s_ks), vs(a[10], s_vs),
+        bt(a[10], s_bt);
+    for (PyObject* o : {bits_o.o, group_o.o, shape.o, kq.o, vq.o, ks.o, vs.o, bt.o})
+        if (o == nullptr) return none();
+    int64_t bits, group, dims[4];
+    if (!as_int(bits_o.o, &bits) || !as_int(group_o.o, &group) || (bits != 4 && bits != 8) || !PyTuple_Check(shape.o) || PyTuple_GET_SIZE(shape.o) != 4)
+        return none();
+    for (int i = 0; i < 4; ++i)
+        if (!as_int(PyTuple_GET_ITEM(shape.o, i), &dims[i])) return none();
+    return append_rows(a, as_tensor(bt.o), as_tensor(kq.o), as_tensor(vq.o), as_tensor(ks.o), as_tensor(vs.o), dims, bits, group);
+}
+
+// norm_rope_append_pages(..., layout, K_pages, V_pages, block_table) -> q or None: plain pages
+PyObject* norm_rope_append_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (p_append == nullptr || n_args != 13) return none();
+    const Tensor *kp = as_tensor(a[10]), *vp = as_tensor(a[11]);
+    if (kp == nullptr || kp->dim() != 4) return none();
+    const int64_t dims[4] = {kp->size(0), kp->size(1), kp->size(2), kp->size(3)};
+    return append_rows(a, as_tensor(a[12]), kp, vp, nullptr, nullptr, dims, 16, 0);
 }
 
 PyObject *s_a, *s_b, *s_scaling, *s_ranks, *s_kz, *s_vz;
@@ -786,6 +807,7 @@ PyMethodDef methods[] = {
     {"dequantize_kv", FAST(dequantize_kv), METH_FASTCALL, nullptr},
     {"head_rope", FAST(head_rope), METH_FASTCALL, nullptr},
     {"norm_rope_append", FAST(norm_rope_append), METH_FASTCALL, nullptr},
+    {"norm_rope_append_pages", FAST(norm_rope_append_pages), METH_FASTCALL, nullptr},
     {"lora_linear", FAST(lora_linear), METH_FASTCALL, nullptr},
     {"reserve_pages", FAST(reserve_pages), METH_FASTCALL, nullptr},
     {"release_sequences", FAST(release_sequences), METH_FASTCALL, nullptr},

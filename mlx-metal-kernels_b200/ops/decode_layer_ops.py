@@ -103,6 +103,9 @@ def norm_rope_kv_append(qkv, cos, sin, positions, paged_qkv, n_heads: int, *, se
 
     A position outside the table appends the k row unturned and is reported by ``_cabi.device_status()`` (event 6); a token whose
     sequence or page does not exist appends nothing (event 7).  Nothing is read on the host, so the call can be captured."""
+    out = _cabi.host().norm_rope_append(qkv, cos, sin, positions, n_heads, sequences, q_weight, k_weight, eps, layout, paged_qkv)
+    if out is not None:
+        return out
     shape = paged_qkv.original_page_shape
     if shape is None:
         raise ValueError("original_page_shape is required to append")

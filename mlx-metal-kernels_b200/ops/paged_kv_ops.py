@@ -163,6 +163,10 @@ def norm_rope_kv_append_pages(qkv, cos, sin, positions, K_pages, V_pages, block_
     """``decode_layer_ops.norm_rope_kv_append`` for plain pages [NUM_PAGES,PAGE_SIZE,Hkv,D] in the dtype of the rows (modified in
     place): q [T, n_heads, D] turned, k (turned) and v written to the slots of their tokens as they are.  The reference's update
     kernels copy the whole cache per token (kernels/paged_kv_cache_update.metal)."""
+    out = _cabi.host().norm_rope_append_pages(qkv, cos, sin, positions, n_heads, sequences, q_weight, k_weight, eps, layout, K_pages, V_pages,
+                                              block_table)
+    if out is not None:
+        return out
     NUM_PAGES, PAGE_SIZE, Hkv, D, _, _ = _validate_page_tensors(K_pages, V_pages, block_table)
     if K_pages.dtype != qkv.dtype or V_pages.dtype != qkv.dtype:
         raise TypeError(f"pages must have the dtype of the rows, got {K_pages.dtype}, {V_pages.dtype} and {qkv.dtype}")

@@ -270,10 +270,6 @@ def head_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float 
 def append_launch(qkv, cos, sin, positions, sequences, block_table, n_heads, weights, eps, layout, kv_bits, k_pages, v_pages, k_scales,
                   v_scales, page_shape, group_size, who):
     """Checks and launch of the append form for both kinds of pages; ``page_shape`` (NUM_PAGES, PAGE_SIZE, Hkv, D)."""
-    out = _cabi.host().norm_rope_append(qkv, cos, sin, positions, sequences, block_table, n_heads, *weights, eps, layout, kv_bits, k_pages,
-                                        v_pages, k_scales, v_scales, group_size, page_shape)
-    if out is not None:
-        return out
     num_pages, page_size, Hkv, D = page_shape
     if qkv.ndim != 2 or qkv.shape[1] != (n_heads + 2 * Hkv) * D or n_heads <= 0:
         raise ValueError(f"qkv must be [T, (n_heads + 2 * {Hkv}) * {D}] with n_heads = {n_heads}, got {tuple(qkv.shape)}")
