@@ -47,7 +47,7 @@ int b200q_version(void);
 const char* b200q_strerror(int code);
 
 /* Reads (and, if reset != 0, clears) the device-side status word.  Kernels record an event there instead of
- * trapping: 1-5 a bounded wait (on a shared-memory barrier or on a peer's flag) ran out, 6 b200q_rope_kv_append
+ * trapping: 1-5 and 11 a bounded wait (on a shared-memory barrier or on a peer's flag) ran out, 6 b200q_rope_kv_append
  * met a position outside the rotary table (the row was left unrotated), 7 it met a position whose block-table
  * entry is unassigned (nothing was appended), 8 a page operator met indices, lengths or counts that it cannot take, 9 it
  * found too few free pages, 10 a row named an adapter that does not exist.  The largest event seen is returned.  Synchronises `stream`.

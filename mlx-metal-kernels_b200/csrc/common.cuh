@@ -43,6 +43,7 @@ enum DeviceEvent : int {
     EV_KV_PAGE_UNASSIGNED = 7,  // rope + append: the block table has no page for the position (nothing appended)
     EV_PAGE_CALL = 8,         // a page operator met indices, lengths or counts it cannot take
     EV_PAGES_EXHAUSTED = 9,   // a page operator found too few free pages (nothing changed)
+    EV_ROPE_RING = 11,        // rope kernel: a bounded wait of its ring ran out
     EV_LORA_ADAPTER = 10,     // a row names an adapter beyond the stack (the row is left without one)
 };
 

@@ -109,6 +109,30 @@ template <int CACHE> __device__ __forceinline__ uint32_t kv_code(float v, float 
     return (uint32_t)(int)(fminf(fmaxf(rintf(__fdiv_rn(v, scale)), -limit), limit) + offset);
 }
 
+// One piece of eight values, as the cache sees them, to codes: rint(v / scale) through the reciprocal, as in the page quantiser
+// (stack.cu) - the same integer unless the quotient lies within 2^-14 of a tie or a value is not finite; those are divided.
+template <int CACHE> __device__ __forceinline__ void store_codes(const float (&v)[8], float scale, uint8_t* codes, int64_t at) {
+    constexpr float magic = 12582912.0f + (CACHE == CACHE_Q8 ? 128.0f : 8.0f);      // 1.5 2^23: adding it rounds to nearest even
+    const float inv = __fdividef(1.0f, scale);
+    uint32_t c[8];
+    float far = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float r = fmaf(v[i], inv, magic);
+        far = fmaxf(far, fabsf(fmaf(v[i], inv, magic - r)));
+        sum = fmaf(v[i], 0.0f, sum);                         // not 0 when a value is not finite
+        c[i] = __float_as_uint(r) & 0xFFu;
+    }
+    if (!(sum == 0.0f) || !(far <= 0.4999f) || !(scale < 1e30f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
+    }
+    if (CACHE == CACHE_Q8)
+        *reinterpret_cast<uint2*>(codes + at) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+    else
+        *reinterpret_cast<uint32_t*>(codes + at / 2) = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12 | c[4] << 16 | c[5] << 20 | c[6] << 24 | c[7] << 28;
+}
+
 // D a power of two from 32 to 256, R a multiple of 16, groups of whole pieces, everything aligned to 16 bytes.
 template <typename T, int LAYOUT, int CACHE, int RUN>
 __global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ? 3 : 4) rope_heads_kernel(const __grid_constant__ RopeParams p, int log_lanes, uint32_t units) {
@@ -148,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ?
     }
     const int pos = live ? p.positions[t] : 0;
     const int seq = CACHE != NO_CACHE && live ? (p.sequences ? p.sequences[t] : (int)t) : 0;
+    const float inv_d = 1.0f / (float)p.D;
     const bool padding = CACHE != NO_CACHE && seq < 0;
     const bool in_table = pos >= 0 && pos < p.table_len;
     const bool rotate = turns && in_table && !padding && live;
@@ -276,34 +301,327 @@ __global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ?
                 const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
                 const int64_t row = row_index * p.heads[kind] + h0 + j;
                 auto store = [&](const float (&v)[8], float scale, int d) {
-                    // rint(v / scale) through the reciprocal, as in the page quantiser (stack.cu): the same integer unless the quotient
-                    // lies within 2^-14 of a tie or is not finite; those pieces are divided
-                    constexpr float magic = 12582912.0f + (CACHE == CACHE_Q8 ? 128.0f : 8.0f);
-                    const float inv = __fdividef(1.0f, scale);
-                    uint32_t c[8];
-                    float far = 0.0f, sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float r = fmaf(v[i], inv, magic);
-                        far = fmaxf(far, fabsf(fmaf(v[i], inv, magic - r)));
-                        sum += v[i] * 0.0f;                  // not zero when a value is not finite
-                        c[i] = __float_as_uint(r) & 0xFFu;
-                    }
-                    if (!(sum == 0.0f) || !(far <= 0.4999f) || !(scale < 1e30f)) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
-                    }
-                    uint8_t* codes = reinterpret_cast<uint8_t*>(p.codes[kind]);
-                    if (CACHE == CACHE_Q8)
-                        *reinterpret_cast<uint2*>(codes + row * p.D + d) =
-                            make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-                    else
-                        *reinterpret_cast<uint32_t*>(codes + (row * p.D + d) / 2) =
-                            c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12 | c[4] << 16 | c[5] << 20 | c[6] << 24 | c[7] << 28;
+                    store_codes<CACHE>(v, scale, reinterpret_cast<uint8_t*>(p.codes[kind]), row * p.D + d);
                     if (d % p.G == 0) p.scales[kind][row * (p.D / p.G) + d / p.G] = __float2half_rn(scale);
                 };
                 store(a, q0, d0);
                 store(b, q1, d1);
+            }
+        }
+    }
+}
+
+// two fp32 values in one 64-bit register, for the packed instructions
+struct f32x2 { unsigned long long v; };
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(f32x2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void halves(uint32_t w, float& lo, float& hi);
+template <> __device__ __forceinline__ void halves<__half>(uint32_t w, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+}
+template <> __device__ __forceinline__ void halves<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+}
+template <typename T> __device__ __forceinline__ uint32_t word(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t word<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t word<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The 16 values of a lane's two pieces as the u and the v of eight pairs: interleaved, each piece has four pairs; else piece 0 is
+// the u and piece 1 the v.
+struct Pairs { f32x2 u[4], v[4]; };
+template <typename T, bool INTERLEAVE> __device__ __forceinline__ Pairs unpack(const uint4& p0, const uint4& p1) {
+    const uint32_t w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) halves<T>(w[i], lo[i], hi[i]);
+    Pairs r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.u[i] = INTERLEAVE ? pair(lo[2 * i], lo[2 * i + 1]) : pair(lo[i], hi[i]);
+        r.v[i] = INTERLEAVE ? pair(hi[2 * i], hi[2 * i + 1]) : pair(lo[4 + i], hi[4 + i]);
+    }
+    return r;
+}
+template <typename T, bool INTERLEAVE> __device__ __forceinline__ void pack(const Pairs& r, uint4& p0, uint4& p1) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float u0, u1, v0, v1;
+        split(r.u[i], u0, u1);
+        split(r.v[i], v0, v1);
+        w[INTERLEAVE ? 2 * i : i] = INTERLEAVE ? word<T>(u0, v0) : word<T>(u0, u1);
+        w[INTERLEAVE ? 2 * i + 1 : 4 + i] = INTERLEAVE ? word<T>(u1, v1) : word<T>(v0, v1);
+    }
+    p0 = make_uint4(w[0], w[1], w[2], w[3]);
+    p1 = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// ---- many tokens: rows through a ring in shared memory ---------------------------------------------------------------------
+// The kernel above has no more bytes in flight than its registers hold.  Here a producer warp copies whole token rows (and their cos / sin
+// rows) into a ring by bulk copies and finds the tokens' slots; consumer threads keep their heads and walk over the tokens.  A lane's two
+// pieces are chosen so that it owns both halves of its pairs; its 16 values are held as two vectors (the u and the v of eight pairs), two
+// values per 64-bit register, for the packed fp32 instructions.
+constexpr int kRingThreads = 384, kMaxStages = 12;
+constexpr uint32_t kRingWaitLimit = 1u << 22;
+constexpr uint32_t kRingBytes = 96 * 1024;      // of a block's stages: two blocks per SM
+constexpr int kRingTokens = 8;                  // per SM, from which on the ring is used
+
+struct RingParams {
+    RopeParams r;
+    uint32_t row_bytes[2];        // of a token: the first run of heads (q, or all of a fused row) and the second (k, or none)
+    uint32_t table_bytes;         // of a row of cos or of sin
+    uint32_t stage_bytes;
+    int stages, consumers;        // consumer threads: lanes of all runs of heads, in whole warps
+};
+struct RingToken {
+    int64_t row;                  // slot in the pool, in tokens, or -1
+    int turn, padding;
+};
+
+template <typename T, bool HALF, int CACHE, int RUN, bool NORM>
+__global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const __grid_constant__ RingParams rp, int log_lanes) {
+    const RopeParams& p = rp.r;
+    constexpr bool kCoded = CACHE == CACHE_Q4 || CACHE == CACHE_Q8;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
+    __shared__ RingToken info[kMaxStages];
+    __shared__ float piece_max[kCoded ? kRingThreads * 2 : 1];
+    const int warps = rp.consumers / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < rp.stages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, warps);
+        }
+        mbar_fence_init();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    __syncthreads();
+    const int64_t n = (p.T - blockIdx.x + gridDim.x - 1) / gridDim.x;        // tokens of this block
+    if (warp == warps) {                                     // ---- producer ----
+        int64_t issued = 0;
+        bool ok = true;
+        int stage = 0;
+        uint32_t parity = 1;                                 // of the empty barriers: the first round finds them free
+        for (int64_t i0 = 0; i0 < n && ok; i0 += 32) {
+            // a lane's token of the next 32
+            const int64_t mine = blockIdx.x + (i0 + lane) * gridDim.x;
+            const bool live = i0 + lane < n;
+            const int pos = live ? p.positions[mine] : 0;
+            const int seq = CACHE != NO_CACHE && live && p.sequences ? p.sequences[mine] : (int)mine;
+            const bool padding = CACHE != NO_CACHE && seq < 0, in_table = pos >= 0 && pos < p.table_len;
+            if (live && !padding && !in_table) atomicMax(&g_device_status, (int)EV_ROPE_POSITION);
+            const int64_t row = CACHE != NO_CACHE && live ? cache_row(p, mine, pos, seq, true) : -1;
+            const int turn = !padding && in_table;
+            for (int k = 0; k < 32 && i0 + k < n; ++k) {
+                if (!mbar_wait_bounded(empty + stage, parity, &g_device_status, EV_ROPE_RING, kRingWaitLimit)) {
+                    ok = false;
+                    break;
+                }
+                const int at = __shfl_sync(0xFFFFFFFFu, pos, k), turns = __shfl_sync(0xFFFFFFFFu, turn, k), pads = __shfl_sync(0xFFFFFFFFu, (int)padding, k);
+                const int64_t slot = __shfl_sync(0xFFFFFFFFu, row, k), t = blockIdx.x + (i0 + k) * gridDim.x;
+                if (lane == 0) {
+                    info[stage] = {slot, turns, pads};
+                    mbar_arrive_expect_tx(full + stage, rp.row_bytes[0] + rp.row_bytes[1] + (turns ? 2 * rp.table_bytes : 0));
+                }
+                __syncwarp();
+                uint8_t* dst = ring + (size_t)stage * rp.stage_bytes;
+                const uint32_t rows = rp.row_bytes[0] + rp.row_bytes[1];
+                if (lane < 2 && rp.row_bytes[lane] > 0)
+                    bulk_g2s(dst + (lane ? rp.row_bytes[0] : 0), reinterpret_cast<const T*>(p.in[lane]) + t * p.in_token[lane], rp.row_bytes[lane], full + stage);
+                if ((lane == 2 || lane == 3) && turns)
+                    bulk_g2s(dst + rows + (lane == 3 ? rp.table_bytes : 0), (lane == 2 ? p.cos_table : p.sin_table) + (int64_t)at * (p.R / 2), rp.table_bytes, full + stage);
+                issued = i0 + k + 1;
+                if (++stage == rp.stages) {
+                    stage = 0;
+                    parity ^= 1u;
+                }
+            }
+        }
+        if (!ok)                                             // the consumers gave up: the copies in flight must land before the block ends
+            for (int64_t i = max((int64_t)0, issued - rp.stages); i < issued; ++i)
+                mbar_wait_bounded(full + i % rp.stages, (uint32_t)(i / rp.stages) & 1u, &g_device_status, EV_ROPE_RING, 1u << 16);
+        return;
+    }
+    // ---- consumers ----
+    const int lanes = 1 << log_lanes, l = threadIdx.x & (lanes - 1);
+    int run = threadIdx.x >> log_lanes, kind = KIND_Q;
+    const bool works = run < p.runs[0] + p.runs[1] + p.runs[2];
+    if (run >= p.runs[0]) { run -= p.runs[0]; kind = KIND_K; }
+    if (kind == KIND_K && run >= p.runs[1]) { run -= p.runs[1]; kind = KIND_V; }
+    const int h0 = run * RUN, count = works ? min(RUN, p.heads[kind] - h0) : 0;
+    // first dimensions of the lane's two pieces: interleaved any two, else the u and the v of eight pairs or two pieces behind R
+    const int half = p.R / 2, l_turns = half / 8;
+    const int d0 = !HALF || l < l_turns ? l * 8 : p.R + (l - l_turns) * 16;
+    const int d1 = !HALF ? (l + lanes) * 8 : l < l_turns ? d0 + half : d0 + 8;
+    const bool has_turn0 = kind != KIND_V && (HALF ? l < l_turns : d0 < p.R), has_turn1 = kind != KIND_V && (HALF ? l < l_turns : d1 < p.R);
+    const int pair0 = HALF ? d0 : d0 / 2, pair1 = HALF ? d0 + 4 : d1 / 2;      // first of four pairs, of c[0..1] and of c[2..3]
+    const int first_head = h0 + (kind == KIND_Q ? 0 : kind == KIND_K ? p.heads[0] : p.heads[0] + p.heads[1]);
+    const uint32_t rows = rp.row_bytes[0] + rp.row_bytes[1];
+    const unsigned group = (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (lane & ~(lanes - 1));
+    const void* weight = NORM && works ? p.weight[kind] : nullptr;
+    Pairs w;
+    if (NORM && weight != nullptr) {
+        float a[8], b[8];
+        load_weight8(weight, p.w_dtype, d0, a);
+        load_weight8(weight, p.w_dtype, d1, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = 4 * (i & 1);
+            w.u[i] = HALF ? pair(a[2 * i], a[2 * i + 1]) : i < 2 ? pair(a[k], a[k + 2]) : pair(b[k], b[k + 2]);
+            w.v[i] = HALF ? pair(b[2 * i], b[2 * i + 1]) : i < 2 ? pair(a[k + 1], a[k + 3]) : pair(b[k + 1], b[k + 3]);
+        }
+    }
+    // where the lane reads in a stage, and where it writes: a row that moves with the token, or the token's row of the pool
+    const uint32_t at0 = ((uint32_t)first_head * p.D + d0) * 2, at1 = ((uint32_t)first_head * p.D + d1) * 2;
+    const uint32_t cos0 = rows + pair0 * 4, cos1 = rows + pair1 * 4;
+    const bool to_pool = CACHE != NO_CACHE && kind != KIND_Q;
+    T* out = to_pool ? reinterpret_cast<T*>(p.codes[kind]) + (kCoded ? 0 : (int64_t)h0 * p.D)
+                     : reinterpret_cast<T*>(p.out[kind]) + blockIdx.x * p.out_token[kind] + (int64_t)h0 * p.out_head[kind];
+    const int64_t out_step = to_pool ? (int64_t)p.heads[kind] * p.D : gridDim.x * p.out_token[kind];
+    const int64_t head_step = to_pool ? p.D : p.out_head[kind];
+    const uint8_t* src = ring;
+    const float inv_d = 1.0f / (float)p.D;
+    int stage = 0;
+    uint32_t parity = 0;
+    for (int i = 0; i < (int)n; ++i) {
+        if (!mbar_wait_bounded(full + stage, parity, &g_device_status, EV_ROPE_RING, kRingWaitLimit)) return;
+        const RingToken token = info[stage];
+        uint4 x0[RUN], x1[RUN];
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) {
+            x0[j] = x1[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (j < count) {
+                x0[j] = *reinterpret_cast<const uint4*>(src + at0 + j * p.D * 2);
+                x1[j] = *reinterpret_cast<const uint4*>(src + at1 + j * p.D * 2);
+            }
+        }
+        const bool turns0 = token.turn && has_turn0, turns1 = token.turn && has_turn1;
+        f32x2 c[4], s[4];
+        {
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a, e = a, f = a;
+            if (turns0) {
+                a = *reinterpret_cast<const float4*>(src + cos0);
+                b = *reinterpret_cast<const float4*>(src + cos0 + rp.table_bytes);
+            }
+            if (turns1) {
+                e = *reinterpret_cast<const float4*>(src + cos1);
+                f = *reinterpret_cast<const float4*>(src + cos1 + rp.table_bytes);
+            }
+            c[0] = pair(a.x, a.y); c[1] = pair(a.z, a.w); c[2] = pair(e.x, e.y); c[3] = pair(e.z, e.w);
+            s[0] = pair(b.x, b.y); s[1] = pair(b.z, b.w); s[2] = pair(f.x, f.y); s[3] = pair(f.z, f.w);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + stage);           // all of the stage is in registers
+        src += rp.stage_bytes;
+        if (++stage == rp.stages) {
+            stage = 0;
+            src = ring;
+            parity ^= 1u;
+        }
+        T* row = to_pool ? out + token.row * out_step : out;
+        out += to_pool ? 0 : out_step;
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) {
+            Pairs x = unpack<T, !HALF>(x0[j], x1[j]);
+            if (NORM && weight != nullptr) {                 // uniform over the lanes of a head
+                f32x2 q = mul2(x.u[0], x.u[0]);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) q = fma2(x.u[k], x.u[k], q);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q = fma2(x.v[k], x.v[k], q);
+                float lo, hi;
+                split(q, lo, hi);
+                float ss = lo + hi;
+                for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(group, ss, o);
+                const float inv = rsqrtf(ss * inv_d + p.eps);      // D is a power of two
+                const f32x2 inv2 = pair(inv, inv);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x.u[k] = mul2(mul2(x.u[k], inv2), w.u[k]);
+                    x.v[k] = mul2(mul2(x.v[k], inv2), w.v[k]);
+                }
+            }
+            // separately rounded products and one sum, as elementwise operations give them (the sums one by one: a packed product and a
+            // packed sum are contracted in spite of their rounding modifiers)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k < 2 ? turns0 : turns1) {
+                    float uc0, uc1, vs0, vs1, us0, us1, vc0, vc1;
+                    split(mul2(x.u[k], c[k]), uc0, uc1);
+                    split(mul2(x.v[k], s[k]), vs0, vs1);
+                    split(mul2(x.u[k], s[k]), us0, us1);
+                    split(mul2(x.v[k], c[k]), vc0, vc1);
+                    x.u[k] = pair(__fsub_rn(uc0, vs0), __fsub_rn(uc1, vs1));
+                    x.v[k] = pair(__fadd_rn(us0, vc0), __fadd_rn(us1, vc1));
+                }
+            }
+            uint4 y0, y1;
+            pack<T, !HALF>(x, y0, y1);
+            if (!kCoded || !to_pool) {
+                if (j < count && (!to_pool || token.row >= 0)) {
+                    if (CACHE != NO_CACHE && token.padding) y0 = y1 = make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(row + j * head_step + d0) = y0;
+                    *reinterpret_cast<uint4*>(row + j * head_step + d1) = y1;
+                }
+            } else if (kCoded) {
+                // the values as the cache sees them, rounded to T; largest magnitudes by piece, then by group of G/8 pieces in order
+                float a[8], b[8], m0 = 0.0f, m1 = 0.0f;
+                const uint32_t e0[4] = {y0.x, y0.y, y0.z, y0.w}, e1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    halves<T>(e0[k], a[2 * k], a[2 * k + 1]);
+                    halves<T>(e1[k], b[2 * k], b[2 * k + 1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    m0 = fmaxf(m0, fabsf(a[k]));
+                    m1 = fmaxf(m1, fabsf(b[k]));
+                }
+                float* of_head = piece_max + (threadIdx.x - l) * 2;
+                __syncwarp(group);
+                of_head[d0 / 8] = m0;
+                of_head[d1 / 8] = m1;
+                __syncwarp(group);
+                if (j < count && token.row >= 0) {
+                    const int pieces = p.G / 8, g0 = d0 / 8 / pieces * pieces, g1 = d1 / 8 / pieces * pieces;
+                    for (int k = 0; k < pieces; ++k) {
+                        m0 = fmaxf(m0, of_head[g0 + k]);
+                        m1 = fmaxf(m1, of_head[g1 + k]);
+                    }
+                    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f;
+                    const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
+                    const int64_t at = token.row * p.heads[kind] + h0 + j;
+                    uint8_t* codes = reinterpret_cast<uint8_t*>(p.codes[kind]);
+                    store_codes<CACHE>(a, q0, codes, at * p.D + d0);
+                    store_codes<CACHE>(b, q1, codes, at * p.D + d1);
+                    __half* scales = p.scales[kind] + at * (p.D / p.G);
+                    if (d0 % p.G == 0) scales[d0 / p.G] = __float2half_rn(q0);
+                    if (d1 % p.G == 0) scales[d1 / p.G] = __float2half_rn(q1);
+                }
             }
         }
     }
@@ -411,6 +729,33 @@ int launch(K kernel, int64_t blocks, int threads, size_t smem, cudaStream_t stre
     return finish_launch();
 }
 
+// Many tokens whose heads are contiguous: the ring kernel; B200Q_ERR_UNSUPPORTED, with nothing launched, for other calls.
+template <typename T, int CACHE>
+int ring(const RopeParams& params, bool half_layout, int log_lanes, cudaStream_t stream) {
+    RingParams rp = {};
+    RopeParams& p = rp.r = params;
+    const bool fused = CACHE != NO_CACHE;
+    const int heads = p.heads[0] + p.heads[1] + p.heads[2], run = (heads << log_lanes) <= kRingThreads ? 1 : 2;
+    if (p.T < kRingTokens * sm_count()) return B200Q_ERR_UNSUPPORTED;
+    for (int i = 0; i < 2; ++i)
+        if (p.heads[i] > 1 && p.in_head[i] != p.D) return B200Q_ERR_UNSUPPORTED;
+    for (int i = 0; i < 3; ++i) p.runs[i] = (p.heads[i] + run - 1) / run;
+    rp.consumers = (((p.runs[0] + p.runs[1] + p.runs[2]) << log_lanes) + 31) / 32 * 32;
+    const uint32_t head_bytes = (uint32_t)p.D * 2;
+    rp.row_bytes[0] = (fused ? heads : p.heads[0]) * head_bytes;
+    rp.row_bytes[1] = fused ? 0 : p.heads[1] * head_bytes;
+    rp.table_bytes = (uint32_t)p.R * 2;
+    rp.stage_bytes = (rp.row_bytes[0] + rp.row_bytes[1] + 2 * rp.table_bytes + 127) / 128 * 128;
+    rp.stages = (int)std::min<uint32_t>(kMaxStages, kRingBytes / rp.stage_bytes);
+    if (rp.consumers > kRingThreads || rp.stages < 3) return B200Q_ERR_UNSUPPORTED;
+    const size_t smem = (size_t)rp.stages * rp.stage_bytes;
+    const bool norm = p.weight[0] != nullptr || p.weight[1] != nullptr;
+    void (*kernel)(const RingParams, int) = half_layout ? (run == 1 ? (norm ? rope_ring_kernel<T, true, CACHE, 1, true> : rope_ring_kernel<T, true, CACHE, 1, false>) : rope_ring_kernel<T, true, CACHE, 2, true>)
+                                                        : (run == 1 ? (norm ? rope_ring_kernel<T, false, CACHE, 1, true> : rope_ring_kernel<T, false, CACHE, 1, false>) : rope_ring_kernel<T, false, CACHE, 2, true>);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    return launch(kernel, std::min<int64_t>(p.T, (int64_t)sm_count() * 2), rp.consumers + 32, smem, stream, rp, log_lanes);
+}
+
 template <typename T, int CACHE>
 int dispatch(RopeParams& p, bool half_layout, cudaStream_t stream) {
     const bool pow2 = (p.D & (p.D - 1)) == 0 && p.D >= 32 && p.D <= 256;
@@ -418,6 +763,8 @@ int dispatch(RopeParams& p, bool half_layout, cudaStream_t stream) {
     if (pow2 && p.R % 16 == 0 && groups && aligned16(p)) {
         int log_lanes = 1;
         while ((16 << log_lanes) < p.D) ++log_lanes;
+        const int rc = ring<T, CACHE>(p, half_layout, log_lanes, stream);
+        if (rc != B200Q_ERR_UNSUPPORTED) return rc;
         // one head per group of lanes while all of them fit the GPU at once (the shortest chain), else two (RUN)
         const int64_t all = p.T * ((int64_t)p.heads[0] + p.heads[1] + p.heads[2]), per_block = kThreads >> log_lanes;
         const int run = all <= (int64_t)sm_count() * 4 * per_block ? 1 : 2;
