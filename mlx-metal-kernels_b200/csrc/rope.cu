@@ -109,28 +109,127 @@ template <int CACHE> __device__ __forceinline__ uint32_t kv_code(float v, float 
     return (uint32_t)(int)(fminf(fmaxf(rintf(__fdiv_rn(v, scale)), -limit), limit) + offset);
 }
 
-// One piece of eight values, as the cache sees them, to codes: rint(v / scale) through the reciprocal, as in the page quantiser
-// (stack.cu) - the same integer unless the quotient lies within 2^-14 of a tie or a value is not finite; those are divided.
-template <int CACHE> __device__ __forceinline__ void store_codes(const float (&v)[8], float scale, uint8_t* codes, int64_t at) {
+// two fp32 values in one 64-bit register, for the packed instructions
+struct f32x2 { unsigned long long v; };
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(f32x2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void halves(uint32_t w, float& lo, float& hi);
+template <> __device__ __forceinline__ void halves<__half>(uint32_t w, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+}
+template <> __device__ __forceinline__ void halves<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+}
+template <typename T> __device__ __forceinline__ uint32_t word(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t word<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t word<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The 16 values of a lane's two pieces as the u and the v of eight pairs: interleaved, each piece has four pairs; else piece 0 is
+// the u and piece 1 the v.
+struct Pairs { f32x2 u[4], v[4]; };
+template <typename T, bool INTERLEAVE> __device__ __forceinline__ Pairs unpack(const uint4& p0, const uint4& p1) {
+    const uint32_t w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) halves<T>(w[i], lo[i], hi[i]);
+    Pairs r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.u[i] = INTERLEAVE ? pair(lo[2 * i], lo[2 * i + 1]) : pair(lo[i], hi[i]);
+        r.v[i] = INTERLEAVE ? pair(hi[2 * i], hi[2 * i + 1]) : pair(lo[4 + i], hi[4 + i]);
+    }
+    return r;
+}
+template <typename T, bool INTERLEAVE> __device__ __forceinline__ void pack(const Pairs& r, uint4& p0, uint4& p1) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float u0, u1, v0, v1;
+        split(r.u[i], u0, u1);
+        split(r.v[i], v0, v1);
+        w[INTERLEAVE ? 2 * i : i] = INTERLEAVE ? word<T>(u0, v0) : word<T>(u0, u1);
+        w[INTERLEAVE ? 2 * i + 1 : 4 + i] = INTERLEAVE ? word<T>(u1, v1) : word<T>(v0, v1);
+    }
+    p0 = make_uint4(w[0], w[1], w[2], w[3]);
+    p1 = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// Largest magnitude of a piece's eight values; NaN when one is.
+template <typename T> __device__ __forceinline__ float piece_top(const uint4& u);
+template <> __device__ __forceinline__ float piece_top<__half>(const uint4& u) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+}
+template <> __device__ __forceinline__ float piece_top<__nv_bfloat16>(const uint4& u) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+}
+// The piece as the cache's rule sees it: its values and their largest magnitude, NaN passed over; `plain`: all are finite.
+template <typename T> __device__ __forceinline__ float piece_values(const uint4& u, float (&v)[8], bool& plain) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) halves<T>(w[i], v[2 * i], v[2 * i + 1]);
+    float top = piece_top<T>(u);
+    plain = top < 3e38f;
+    if (!plain) {
+        top = 0.0f;
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    }
+    return top;
+}
+// max(top, 1e-8) / (127 | 7), correctly rounded: one correction of the product with the reciprocal is enough between 1e-8 and 3e38
+template <int CACHE> __device__ __forceinline__ float group_scale(float top) {
+    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f, inv = 1.0f / limit;
+    const float m = fmaxf(top, 1e-8f);
+    if (!(m < 3e38f)) return __fdiv_rn(m, limit);
+    const float q = m * inv;
+    return fmaf(fmaf(-q, limit, m), inv, q);
+}
+// Its codes: rint(v / scale) through the reciprocal, as in the page quantiser (stack.cu) - the same integer unless the quotient
+// lies within 2^-14 of a tie, or something is not finite; those are divided.
+template <int CACHE> __device__ __forceinline__ void store_codes(const float (&v)[8], float scale, bool plain, uint8_t* codes) {
     constexpr float magic = 12582912.0f + (CACHE == CACHE_Q8 ? 128.0f : 8.0f);      // 1.5 2^23: adding it rounds to nearest even
     const float inv = __fdividef(1.0f, scale);
     uint32_t c[8];
-    float far = 0.0f, sum = 0.0f;
+    float far = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float r = fmaf(v[i], inv, magic);
         far = fmaxf(far, fabsf(fmaf(v[i], inv, magic - r)));
-        sum = fmaf(v[i], 0.0f, sum);                         // not 0 when a value is not finite
-        c[i] = __float_as_uint(r) & 0xFFu;
+        c[i] = __float_as_uint(r);
     }
-    if (!(sum == 0.0f) || !(far <= 0.4999f) || !(scale < 1e30f)) {
+    if (!plain || !(far <= 0.4999f) || !(scale < 1e30f)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
     }
-    if (CACHE == CACHE_Q8)
-        *reinterpret_cast<uint2*>(codes + at) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-    else
-        *reinterpret_cast<uint32_t*>(codes + at / 2) = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12 | c[4] << 16 | c[5] << 20 | c[6] << 24 | c[7] << 28;
+    auto bytes = [](uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) { return prmt(prmt(c0, c1, 0x0040u), prmt(c2, c3, 0x0040u), 0x5410u); };
+    if (CACHE == CACHE_Q8) *reinterpret_cast<uint2*>(codes) = make_uint2(bytes(c[0], c[1], c[2], c[3]), bytes(c[4], c[5], c[6], c[7]));
+    else *reinterpret_cast<uint32_t*>(codes) = bytes(c[0], c[2], c[4], c[6]) | bytes(c[1], c[3], c[5], c[7]) << 4;
 }
 
 // D a power of two from 32 to 256, R a multiple of 16, groups of whole pieces, everything aligned to 16 bytes.
@@ -281,14 +380,8 @@ __global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ?
         } else {
             // the values as the cache sees them: rounded to T.  Group maxima over the G/8 neighbouring lanes; a group of the
             // whole head takes both pieces of every lane
-            unpack8(y0, a, (const T*)nullptr);
-            unpack8(y1, b, (const T*)nullptr);
-            float m0 = 0.0f, m1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                m0 = fmaxf(m0, fabsf(a[i]));
-                m1 = fmaxf(m1, fabsf(b[i]));
-            }
+            bool plain0, plain1;
+            float m0 = piece_values<T>(y0, a, plain0), m1 = piece_values<T>(y1, b, plain1);
             const int pieces = p.G / 8;
             if (pieces > lanes) m0 = m1 = fmaxf(m0, m1);
             const unsigned group = (lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u)) << (threadIdx.x & 31 & ~(lanes - 1));
@@ -297,88 +390,19 @@ __global__ void __launch_bounds__(kThreads, RUN == 1 ? 1 : LAYOUT == HALF_PART ?
                 m1 = fmaxf(m1, __shfl_xor_sync(group, m1, o));
             }
             if (j < count && row_index >= 0) {
-                constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f;
-                const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
+                const float q0 = group_scale<CACHE>(m0), q1 = group_scale<CACHE>(m1);
                 const int64_t row = row_index * p.heads[kind] + h0 + j;
-                auto store = [&](const float (&v)[8], float scale, int d) {
-                    store_codes<CACHE>(v, scale, reinterpret_cast<uint8_t*>(p.codes[kind]), row * p.D + d);
+                auto store = [&](const float (&v)[8], float scale, bool plain, int d) {
+                    store_codes<CACHE>(v, scale, plain, reinterpret_cast<uint8_t*>(p.codes[kind]) + (row * p.D + d) / (CACHE == CACHE_Q4 ? 2 : 1));
                     if (d % p.G == 0) p.scales[kind][row * (p.D / p.G) + d / p.G] = __float2half_rn(scale);
                 };
-                store(a, q0, d0);
-                store(b, q1, d1);
+                store(a, q0, plain0, d0);
+                store(b, q1, plain1, d1);
             }
         }
     }
 }
 
-// two fp32 values in one 64-bit register, for the packed instructions
-struct f32x2 { unsigned long long v; };
-__device__ __forceinline__ f32x2 pair(float lo, float hi) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void split(f32x2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-
-template <typename T> __device__ __forceinline__ void halves(uint32_t w, float& lo, float& hi);
-template <> __device__ __forceinline__ void halves<__half>(uint32_t w, float& lo, float& hi) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    lo = f.x;
-    hi = f.y;
-}
-template <> __device__ __forceinline__ void halves<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
-    lo = __uint_as_float(w << 16);
-    hi = __uint_as_float(w & 0xFFFF0000u);
-}
-template <typename T> __device__ __forceinline__ uint32_t word(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t word<__half>(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t word<__nv_bfloat16>(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// The 16 values of a lane's two pieces as the u and the v of eight pairs: interleaved, each piece has four pairs; else piece 0 is
-// the u and piece 1 the v.
-struct Pairs { f32x2 u[4], v[4]; };
-template <typename T, bool INTERLEAVE> __device__ __forceinline__ Pairs unpack(const uint4& p0, const uint4& p1) {
-    const uint32_t w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-    float lo[8], hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) halves<T>(w[i], lo[i], hi[i]);
-    Pairs r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r.u[i] = INTERLEAVE ? pair(lo[2 * i], lo[2 * i + 1]) : pair(lo[i], hi[i]);
-        r.v[i] = INTERLEAVE ? pair(hi[2 * i], hi[2 * i + 1]) : pair(lo[4 + i], hi[4 + i]);
-    }
-    return r;
-}
-template <typename T, bool INTERLEAVE> __device__ __forceinline__ void pack(const Pairs& r, uint4& p0, uint4& p1) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float u0, u1, v0, v1;
-        split(r.u[i], u0, u1);
-        split(r.v[i], v0, v1);
-        w[INTERLEAVE ? 2 * i : i] = INTERLEAVE ? word<T>(u0, v0) : word<T>(u0, u1);
-        w[INTERLEAVE ? 2 * i + 1 : 4 + i] = INTERLEAVE ? word<T>(u1, v1) : word<T>(v0, v1);
-    }
-    p0 = make_uint4(w[0], w[1], w[2], w[3]);
-    p1 = make_uint4(w[4], w[5], w[6], w[7]);
-}
 // ---- many tokens: rows through a ring in shared memory ---------------------------------------------------------------------
 // The kernel above has no more bytes in flight than its registers hold.  Here a producer warp copies whole token rows (and their cos / sin
 // rows) into a ring by bulk copies and finds the tokens' slots; consumer threads keep their heads and walk over the tokens.  A lane's two
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const _
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
     __shared__ RingToken info[kMaxStages];
-    __shared__ float piece_max[kCoded ? kRingThreads * 2 : 1];
+    __shared__ __align__(16) float piece_max[kCoded ? kRingThreads * 2 : 1];
     const int warps = rp.consumers / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < rp.stages; ++i) {
@@ -499,10 +523,18 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const _
     const uint32_t at0 = ((uint32_t)first_head * p.D + d0) * 2, at1 = ((uint32_t)first_head * p.D + d1) * 2;
     const uint32_t cos0 = rows + pair0 * 4, cos1 = rows + pair1 * 4;
     const bool to_pool = CACHE != NO_CACHE && kind != KIND_Q;
-    T* out = to_pool ? reinterpret_cast<T*>(p.codes[kind]) + (kCoded ? 0 : (int64_t)h0 * p.D)
+    T* out = to_pool ? reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(p.codes[kind]) + (int64_t)h0 * p.D * (kCoded ? 1 : 2) / (CACHE == CACHE_Q4 ? 2 : 1))
                      : reinterpret_cast<T*>(p.out[kind]) + blockIdx.x * p.out_token[kind] + (int64_t)h0 * p.out_head[kind];
     const int64_t out_step = to_pool ? (int64_t)p.heads[kind] * p.D : gridDim.x * p.out_token[kind];
     const int64_t head_step = to_pool ? p.D : p.out_head[kind];
+    // codes: the groups of the lane's pieces, and its bytes of a head
+    float* of_head = piece_max + (kCoded ? (threadIdx.x - l) * 2 : 0);
+    const int pieces = p.G / 8, groups = p.D / p.G, g0 = d0 / 8 / pieces * pieces, g1 = d1 / 8 / pieces * pieces;
+    const bool leads0 = d0 % p.G == 0, leads1 = d1 % p.G == 0;
+    const int s0_at = d0 / p.G, s1_at = d1 / p.G;
+    constexpr int kPerByte = CACHE == CACHE_Q4 ? 2 : 1;
+    const int code_head = p.D / kPerByte, code0 = d0 / kPerByte, code1 = d1 / kPerByte;
+    const int64_t code_step = (int64_t)p.heads[kind] * code_head;
     const uint8_t* src = ring;
     const float inv_d = 1.0f / (float)p.D;
     int stage = 0;
@@ -589,38 +621,31 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const _
                 }
             } else if (kCoded) {
                 // the values as the cache sees them, rounded to T; largest magnitudes by piece, then by group of G/8 pieces in order
-                float a[8], b[8], m0 = 0.0f, m1 = 0.0f;
-                const uint32_t e0[4] = {y0.x, y0.y, y0.z, y0.w}, e1[4] = {y1.x, y1.y, y1.z, y1.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    halves<T>(e0[k], a[2 * k], a[2 * k + 1]);
-                    halves<T>(e1[k], b[2 * k], b[2 * k + 1]);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    m0 = fmaxf(m0, fabsf(a[k]));
-                    m1 = fmaxf(m1, fabsf(b[k]));
-                }
-                float* of_head = piece_max + (threadIdx.x - l) * 2;
+                float a[8], b[8];
+                bool plain0, plain1;
+                float m0 = piece_values<T>(y0, a, plain0), m1 = piece_values<T>(y1, b, plain1);
                 __syncwarp(group);
                 of_head[d0 / 8] = m0;
                 of_head[d1 / 8] = m1;
                 __syncwarp(group);
                 if (j < count && token.row >= 0) {
-                    const int pieces = p.G / 8, g0 = d0 / 8 / pieces * pieces, g1 = d1 / 8 / pieces * pieces;
-                    for (int k = 0; k < pieces; ++k) {
-                        m0 = fmaxf(m0, of_head[g0 + k]);
-                        m1 = fmaxf(m1, of_head[g1 + k]);
+                    if (pieces >= 4) {
+                        for (int k = 0; k < pieces; k += 4) {
+                            const float4 e = *reinterpret_cast<const float4*>(of_head + g0 + k), f = *reinterpret_cast<const float4*>(of_head + g1 + k);
+                            m0 = fmaxf(fmaxf(fmaxf(m0, e.x), fmaxf(e.y, e.z)), e.w);
+                            m1 = fmaxf(fmaxf(fmaxf(m1, f.x), fmaxf(f.y, f.z)), f.w);
+                        }
+                    } else if (pieces == 2) {
+                        m0 = fmaxf(of_head[g0], of_head[g0 + 1]);
+                        m1 = fmaxf(of_head[g1], of_head[g1 + 1]);
                     }
-                    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f;
-                    const float q0 = __fdiv_rn(fmaxf(m0, 1e-8f), limit), q1 = __fdiv_rn(fmaxf(m1, 1e-8f), limit);
-                    const int64_t at = token.row * p.heads[kind] + h0 + j;
-                    uint8_t* codes = reinterpret_cast<uint8_t*>(p.codes[kind]);
-                    store_codes<CACHE>(a, q0, codes, at * p.D + d0);
-                    store_codes<CACHE>(b, q1, codes, at * p.D + d1);
-                    __half* scales = p.scales[kind] + at * (p.D / p.G);
-                    if (d0 % p.G == 0) scales[d0 / p.G] = __float2half_rn(q0);
-                    if (d1 % p.G == 0) scales[d1 / p.G] = __float2half_rn(q1);
+                    const float q0 = group_scale<CACHE>(m0), q1 = group_scale<CACHE>(m1);
+                    uint8_t* codes = reinterpret_cast<uint8_t*>(out) + token.row * code_step + j * code_head;
+                    store_codes<CACHE>(a, q0, plain0, codes + code0);
+                    store_codes<CACHE>(b, q1, plain1, codes + code1);
+                    __half* scales = p.scales[kind] + (token.row * p.heads[kind] + h0 + j) * groups;
+                    if (leads0) scales[s0_at] = __float2half_rn(q0);
+                    if (leads1) scales[s1_at] = __float2half_rn(q1);
                 }
             }
         }
