@@ -210,22 +210,23 @@ template <int CACHE> __device__ __forceinline__ float group_scale(float top) {
     const float q = m * inv;
     return fmaf(fmaf(-q, limit, m), inv, q);
 }
-// Its codes: rint(v / scale) through the reciprocal, as in the page quantiser (stack.cu) - the same integer unless the quotient
-// lies within 2^-14 of a tie, or something is not finite; those are divided.
+// Its codes.  rint(v / scale) with the quotient rounded as a division rounds it: the product with the correctly rounded reciprocal,
+// corrected once by its exact remainder, is the correctly rounded quotient (Markstein's theorem) wherever it is large enough to matter.
 template <int CACHE> __device__ __forceinline__ void store_codes(const float (&v)[8], float scale, bool plain, uint8_t* codes) {
-    constexpr float magic = 12582912.0f + (CACHE == CACHE_Q8 ? 128.0f : 8.0f);      // 1.5 2^23: adding it rounds to nearest even
-    const float inv = __fdividef(1.0f, scale);
+    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f, offset = CACHE == CACHE_Q8 ? 128.0f : 8.0f;
+    constexpr float magic = 12582912.0f + offset;            // 1.5 2^23: adding it rounds to nearest even and leaves the code in the low byte
+    constexpr uint32_t lowest = (uint32_t)(offset - limit), zero = (uint32_t)offset;
+    const float inv = __frcp_rn(scale);
     uint32_t c[8];
-    float far = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float r = fmaf(v[i], inv, magic);
-        far = fmaxf(far, fabsf(fmaf(v[i], inv, magic - r)));
-        c[i] = __float_as_uint(r);
+        const float q = v[i] * inv;
+        c[i] = __float_as_uint(fmaf(fmaf(-q, scale, v[i]), inv, q) + magic);
     }
-    if (!plain || !(far <= 0.4999f) || !(scale < 1e30f)) {
+    if (!plain || !(scale < INFINITY)) {                     // as the rule has it: NaN becomes the lowest code, and beside an infinity all is zero
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = kv_code<CACHE>(v[i], scale);
+        for (int i = 0; i < 8; ++i)
+            if (!(scale < INFINITY) || !(v[i] == v[i])) c[i] = fabsf(v[i]) < INFINITY ? zero : lowest;
     }
     auto bytes = [](uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) { return prmt(prmt(c0, c1, 0x0040u), prmt(c2, c3, 0x0040u), 0x5410u); };
     if (CACHE == CACHE_Q8) *reinterpret_cast<uint2*>(codes) = make_uint2(bytes(c[0], c[1], c[2], c[3]), bytes(c[4], c[5], c[6], c[7]));
@@ -530,6 +531,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const _
     // codes: the groups of the lane's pieces, and its bytes of a head
     float* of_head = piece_max + (kCoded ? (threadIdx.x - l) * 2 : 0);
     const int pieces = p.G / 8, groups = p.D / p.G, g0 = d0 / 8 / pieces * pieces, g1 = d1 / 8 / pieces * pieces;
+    const bool in_order = !HALF || p.R == p.D;
     const bool leads0 = d0 % p.G == 0, leads1 = d1 % p.G == 0;
     const int s0_at = d0 / p.G, s1_at = d1 / p.G;
     constexpr int kPerByte = CACHE == CACHE_Q4 ? 2 : 1;
@@ -624,21 +626,23 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) rope_ring_kernel(const _
                 float a[8], b[8];
                 bool plain0, plain1;
                 float m0 = piece_values<T>(y0, a, plain0), m1 = piece_values<T>(y1, b, plain1);
-                __syncwarp(group);
-                of_head[d0 / 8] = m0;
-                of_head[d1 / 8] = m1;
-                __syncwarp(group);
-                if (j < count && token.row >= 0) {
-                    if (pieces >= 4) {
-                        for (int k = 0; k < pieces; k += 4) {
-                            const float4 e = *reinterpret_cast<const float4*>(of_head + g0 + k), f = *reinterpret_cast<const float4*>(of_head + g1 + k);
-                            m0 = fmaxf(fmaxf(fmaxf(m0, e.x), fmaxf(e.y, e.z)), e.w);
-                            m1 = fmaxf(fmaxf(fmaxf(m1, f.x), fmaxf(f.y, f.z)), f.w);
-                        }
-                    } else if (pieces == 2) {
-                        m0 = fmaxf(of_head[g0], of_head[g0 + 1]);
-                        m1 = fmaxf(of_head[g1], of_head[g1 + 1]);
+                if (in_order) {                              // pieces l and l + lanes: the lanes of a group are neighbours
+                    if (pieces > lanes) m0 = m1 = fmaxf(m0, m1);
+                    for (int o = 1; o < min(pieces, lanes); o <<= 1) {
+                        m0 = fmaxf(m0, __shfl_xor_sync(group, m0, o));
+                        m1 = fmaxf(m1, __shfl_xor_sync(group, m1, o));
                     }
+                } else {
+                    __syncwarp(group);
+                    of_head[d0 / 8] = m0;
+                    of_head[d1 / 8] = m1;
+                    __syncwarp(group);
+                    for (int k = 0; k < pieces; ++k) {
+                        m0 = fmaxf(m0, of_head[g0 + k]);
+                        m1 = fmaxf(m1, of_head[g1 + k]);
+                    }
+                }
+                if (j < count && token.row >= 0) {
                     const float q0 = group_scale<CACHE>(m0), q1 = group_scale<CACHE>(m1);
                     uint8_t* codes = reinterpret_cast<uint8_t*>(out) + token.row * code_step + j * code_head;
                     store_codes<CACHE>(a, q0, plain0, codes + code0);

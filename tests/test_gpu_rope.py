@@ -353,3 +353,91 @@ def test_streams_and_graphs(cuda):
         for b in range(3):
             page, slot = int(table[b, at[b] // P]), int(at[b] % P)
             assert torch.equal(p[page, slot], q[page, slot])
+
+
+def many(cuda):
+    """Tokens from which on the ring kernel runs (eight per SM), and then some."""
+    return 8 * torch.cuda.get_device_properties(cuda).multi_processor_count + 37
+
+
+@pytest.mark.parametrize("D,R,Hq,Hkv", [(128, 128, 8, 2), (128, 64, 5, 3), (64, 64, 7, 1), (256, 32, 9, 2), (32, 32, 3, 0), (64, 16, 64, 8)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_tokens(cuda, D, R, Hq, Hkv, layout, dtype):
+    """Without norms the bits of calls of few tokens, in place too; with norms the formula's values."""
+    T = many(cuda)
+    g = gen(D + R)
+    qkv = torch.randn((T, Hq + Hkv + 1, D), generator=g).to(dtype)
+    pos = torch.randint(-3, 70, (T,), generator=g, dtype=torch.int32)
+    cos, sin = tables(R)
+    dev = qkv.to(cuda)
+    q, k = dev[:, :Hq], dev[:, Hq:Hq + Hkv] if Hkv else None
+    args = (cos.to(cuda), sin.to(cuda), pos.to(cuda))
+    cabi.device_status()
+    got = rope_ops.apply_rope(q, k, *args, layout=layout)
+    assert cabi.device_status() == 6
+    for x, y in ((q, got[0]), (k, got[1])):
+        if x is not None:
+            few = [rope_ops.apply_rope(x[i:i + 64], None, *args[:2], args[2][i:i + 64], layout=layout)[0] for i in range(0, T, 64)]
+            assert torch.equal(y, torch.cat(few))
+    w = (1 + 0.2 * torch.randn(D, generator=g))
+    normed = rope_ops.head_norm_rope(q, k, w.to(cuda), None, *args, eps=EPS, layout=layout)
+    want, size = want64(qkv[:, :Hq], w, cos, sin, pos, layout)
+    assert_close(normed[0], want, size, dtype, True, D)
+    if k is not None:
+        assert torch.equal(normed[1], got[1])
+    rest = dev[:, Hq + Hkv:].clone()
+    rope_ops.apply_rope(q, k, *args, layout=layout, inplace=True)
+    assert torch.equal(q, got[0]) and (k is None or torch.equal(k, got[1])) and torch.equal(dev[:, Hq + Hkv:], rest)
+    assert cabi.device_status() == 6
+
+
+@pytest.mark.parametrize("bits,D,R,G,layout", [(8, 128, 128, 32, "half"), (4, 128, 128, 32, "interleaved"), (8, 128, 64, 64, "half"), (4, 64, 32, 16, "half"),
+                                               (8, 256, 256, 256, "interleaved"), (8, 128, 128, 8, "half"), (16, 128, 128, 32, "half"), (16, 64, 32, 8, "interleaved")])
+def test_append_of_many_tokens(cuda, bits, D, R, G, layout):
+    """The bits of appends of few tokens: rows, codes, scales, padding, tokens without a page, values that are not finite."""
+    T, P, Hq, Hkv, dtype = many(cuda), 16, 6, 2, torch.bfloat16
+    g = gen(bits + D)
+    B, blocks = 5, (T + 4) // 5 // P + 2
+    pages = B * blocks + 3
+    order = torch.randperm(pages, generator=g)[:B * blocks].to(torch.int32).reshape(B, blocks)
+    order[2, 1] = -1
+    seq = torch.arange(T, dtype=torch.int32) % B
+    pos = (torch.arange(T, dtype=torch.int32) // B) + 3
+    seq[7::50] = -1
+    seq[9] = B
+    qkv = torch.randn((T, Hq + 2 * Hkv, D), generator=g).to(dtype)
+    qkv[3, Hq, 5], qkv[4, Hq + 1, 0], qkv[5, Hq + Hkv, 1], qkv[6, Hq, 3] = float("nan"), float("inf"), float("-inf"), float("nan")
+    qkv[8, Hq:] = 0.0
+    qkv[10, Hq:] = 1e-12
+    qkv = qkv.reshape(T, -1).to(cuda)
+    cos, sin = (t.to(cuda) for t in tables(R, int(pos.max()) + 1))
+    table, seq, pos = order.to(cuda), seq.to(cuda), pos.to(cuda)
+    results = []
+    for step in (T, 64):
+        cache = make_cache(bits if bits < 16 else 8, pages, P, Hkv, D, G, order, torch.zeros(B, dtype=torch.int32), cuda, 7)
+        plain = [torch.full((pages, P, Hkv, D), 2.0, dtype=dtype, device=cuda) for _ in range(2)]
+        out = []
+        for i in range(0, T, step):
+            part = (qkv[i:i + step], cos, sin, pos[i:i + step])
+            if bits == 16:
+                out.append(pkv_ops.norm_rope_kv_append_pages(*part, *plain, table, Hq, sequences=seq[i:i + step], layout=layout))
+            else:
+                out.append(layer_ops.norm_rope_kv_append(*part, cache, Hq, sequences=seq[i:i + step], layout=layout))
+        assert cabi.device_status() == 7
+        pool = plain if bits == 16 else [cache.k_pages_q, cache.v_pages_q, cache.k_scales, cache.v_scales]
+        results.append([torch.cat(out)] + pool)
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert bool((results[0][0][7::50] == 0).all())
+    if bits < 16:                                            # and the rule's codes, also for what is not finite
+        rows = qkv.reshape(T, -1, D)
+        for name, heads in (("v", rows[:, Hq + Hkv:]),):
+            for t in (3, 4, 5, 6, 8, 10, 100, T - 1):
+                if int(seq[t]) < 0:
+                    continue
+                page, slot = int(table[seq[t], pos[t] // P]), int(pos[t] % P)
+                if page < 0:
+                    continue
+                codes, scales = pq_ops._quantize_groups(heads[t].contiguous(), bits, G)
+                assert torch.equal(results[0][2][page, slot], codes) and torch.equal(results[0][4][page, slot].view(torch.uint8), scales.view(torch.uint8))
