@@ -259,11 +259,16 @@ template <int BITS, int LOGG> struct I8Shape {
     static constexpr int XU = GU * 96 * NM;                  // digit bytes of a unit: 1536 (q4) or 768 (q8)
 };
 
+// What a kernel is compiled for: plain rows, packets of a tensor-parallel exchange, or fp32 rows added before the rounding (deciding on
+// the latter at run time made every other call 2 % longer: 4.62 -> 4.71 us for 4096 x 4096 q4).
+enum I8Mode : int { kI8Plain = 0, kI8Packets = 1, kI8Adds = 2 };
+
 // PB: bytes of a piece of scales, 16, 8 or 4, where rows of scales (and the units in them) start at multiples of it: pieces then lie in
 // shared memory as the affine step wants them, eight groups to a load.  0: rows that start anywhere; an aligned window is copied and read
 // one value at a time.  KS: CTAs per row, 1 or 2.  (PB at run time: 3 % slower.)
-template <int BITS, int LOGG, int NB, bool PACKETS, int PB, int KS>
+template <int BITS, int LOGG, int NB, I8Mode MODE, int PB, int KS>
 __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_constant__ I8Params p) {
+    constexpr bool PACKETS = MODE == kI8Packets, ADDS = MODE == kI8Adds;
     extern __shared__ __align__(128) uint8_t smem[];
     using S = I8Shape<BITS, LOGG>;
     constexpr int G = S::G, GB = S::GB, NM = S::NM, GU = S::GU, CP = S::CP, CH = S::CH, CG = S::CG, MB = S::MB, WIN = S::WIN;
@@ -366,13 +371,12 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
         if ((int)threadIdx.x < p.tp_in.world && !tp_wait_source(p.tp_in, threadIdx.x)) atomicMax(&g_device_status, (int)EV_PEER_WAIT);
         __syncthreads();
     }
-    const bool res_smem = (p.residual != nullptr || p.add32 != nullptr) && r_cnt * B <= kI8MaxRes;
+    const bool res_smem = (ADDS || p.residual != nullptr) && r_cnt * B <= kI8MaxRes;
     if (res_smem)
         for (int i = threadIdx.x; i < r_cnt * B; i += kI8Threads) {
             const int b = i / r_cnt;
-            const size_t o = (size_t)b * p.N + r_lo + (i - b * r_cnt);
-            if (p.add32 != nullptr) add[i] = p.add32[o];
-            else resid[i] = reinterpret_cast<const uint16_t*>(p.residual)[o];
+            if constexpr (ADDS) add[i] = p.add32[(size_t)b * p.N + r_lo + (i - b * r_cnt)];
+            else resid[i] = reinterpret_cast<const uint16_t*>(p.residual)[(size_t)b * p.N + r_lo + (i - b * r_cnt)];
         }
     // Items: 8-value pieces of the padded rows.  A warp's 32 pieces lie in one row (a padded row is a multiple of 32 pieces).
     // The loop stays small on purpose: hoisting four loads per thread made every launch 0.4 us longer (instruction fetch)
@@ -629,8 +633,8 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                 float sum = 0.0f;
 #pragma unroll 8
                 for (int i = 0; i < p.units; ++i) sum += src[(m * p.units + i) * (16 * NB)];
-                const float c = fminf(fmaxf(sum, -fmax_act), fmax_act);
-                val[m] = p.add32 != nullptr ? c : i8_round_act(c, p.act_dtype);
+                if constexpr (ADDS) val[m] = fminf(fmaxf(sum, -fmax_act), fmax_act);
+                else val[m] = i8_round_act(fminf(fmaxf(sum, -fmax_act), fmax_act), p.act_dtype);
             }
             const int row = r_lo + rb0 + rr;
             const int64_t o = (int64_t)b * p.N + row;
@@ -644,11 +648,11 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                 v = (val[0] / (1.0f + expf(-val[0]))) * val[1];
                 if (p.act_out != nullptr) reinterpret_cast<unsigned short*>(p.act_out)[o] = bits_of(v);
             } else {
-                if (p.residual != nullptr) {
+                if constexpr (ADDS) {
+                    v = (res_smem ? add[b * r_cnt + rb0 + rr] : p.add32[o]) + v;
+                } else if (p.residual != nullptr) {
                     const uint16_t rb = res_smem ? resid[b * r_cnt + rb0 + rr] : reinterpret_cast<const uint16_t*>(p.residual)[o];
                     v = load_as_f32(&rb, p.act_dtype, 0) + v;
-                } else if (p.add32 != nullptr) {
-                    v = (res_smem ? add[b * r_cnt + rb0 + rr] : p.add32[o]) + v;
                 }
                 if (p.y != nullptr) reinterpret_cast<unsigned short*>(p.y)[o] = bits_of(v);
             }
@@ -753,18 +757,15 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
     if (off > (uint32_t)max_smem_optin()) return B200Q_ERR_UNSUPPORTED;
 
     using KernelFn = void (*)(I8Params);
-    static const KernelFn kernels[4][4] = {
-        {qgemv_i8_kernel<BITS, LOGG, NB, false, 0, 1>, qgemv_i8_kernel<BITS, LOGG, NB, false, P4, 1>,
-         qgemv_i8_kernel<BITS, LOGG, NB, false, P8, 1>, qgemv_i8_kernel<BITS, LOGG, NB, false, P16, 1>},
-        {qgemv_i8_kernel<BITS, LOGG, NB, true, 0, 1>, qgemv_i8_kernel<BITS, LOGG, NB, true, P4, 1>,
-         qgemv_i8_kernel<BITS, LOGG, NB, true, P8, 1>, qgemv_i8_kernel<BITS, LOGG, NB, true, P16, 1>},
-        {qgemv_i8_kernel<BITS, LOGG, NB, false, 0, 2>, qgemv_i8_kernel<BITS, LOGG, NB, false, P4, 2>,
-         qgemv_i8_kernel<BITS, LOGG, NB, false, P8, 2>, qgemv_i8_kernel<BITS, LOGG, NB, false, P16, 2>},
-        {qgemv_i8_kernel<BITS, LOGG, NB, true, 0, 2>, qgemv_i8_kernel<BITS, LOGG, NB, true, P4, 2>,
-         qgemv_i8_kernel<BITS, LOGG, NB, true, P8, 2>, qgemv_i8_kernel<BITS, LOGG, NB, true, P16, 2>}};
-    const int kind = (ks - 1) * 2 + packets;
+#define B200Q_I8_FORMS(MODE, KS)                                                                        \
+    {qgemv_i8_kernel<BITS, LOGG, NB, MODE, 0, KS>, qgemv_i8_kernel<BITS, LOGG, NB, MODE, P4, KS>,       \
+     qgemv_i8_kernel<BITS, LOGG, NB, MODE, P8, KS>, qgemv_i8_kernel<BITS, LOGG, NB, MODE, P16, KS>}
+    static const KernelFn kernels[6][4] = {B200Q_I8_FORMS(kI8Plain, 1), B200Q_I8_FORMS(kI8Packets, 1), B200Q_I8_FORMS(kI8Adds, 1),
+                                           B200Q_I8_FORMS(kI8Plain, 2), B200Q_I8_FORMS(kI8Packets, 2), B200Q_I8_FORMS(kI8Adds, 2)};
+#undef B200Q_I8_FORMS
+    const int kind = (ks - 1) * 3 + (q.add32 != nullptr ? kI8Adds : packets ? kI8Packets : kI8Plain);
     KernelFn kernel = kernels[kind][form];
-    static bool configured[16][64] = {};   // per instantiation and device; a race only repeats the call
+    static bool configured[24][64] = {};   // per instantiation and device; a race only repeats the call
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[kind * 4 + form][dev & 63]) {

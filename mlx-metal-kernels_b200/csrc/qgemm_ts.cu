@@ -39,6 +39,7 @@
 #include "tensor_map.cuh"
 
 #include <algorithm>
+#include <type_traits>
 #include <functional>
 #include <mutex>
 #include <unordered_map>
@@ -305,19 +306,22 @@ __device__ __forceinline__ float ts_float(bool bf, uint16_t u) {
 }
 // The residual values of output row n for 4 columns, fetched ahead of the accumulators and before the first store (y may
 // alias the residual rows as far as the compiler knows).
-template <int MATS>
-__device__ __forceinline__ void ts_load_residual(const TsParams& p, int n, int b0, int nb, uint32_t (&res)[4]) {
+template <bool ADD> using TsRes = std::conditional_t<ADD, float, uint16_t>;
+template <int MATS, bool ADD>
+__device__ __forceinline__ void ts_load_residual(const TsParams& p, int n, int b0, int nb, TsRes<ADD> (&res)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         res[j] = 0;
-        if (MATS != 1 || n >= p.N || j >= nb) continue;
-        if (p.residual != nullptr) res[j] = p.residual[(size_t)(b0 + j) * p.N + n];
-        else if (p.add32 != nullptr) res[j] = __float_as_uint(p.add32[(size_t)(b0 + j) * p.N + n]);
+        if constexpr (ADD) {
+            if (n < p.N && j < nb) res[j] = p.add32[(size_t)(b0 + j) * p.N + n];
+        } else {
+            if (MATS == 1 && p.residual != nullptr && n < p.N && j < nb) res[j] = p.residual[(size_t)(b0 + j) * p.N + n];
+        }
     }
 }
 // The epilogue of 4 columns (b0 .. b0 + nb of the batch): clamp, round, residual add or SwiGLU, store.
-template <int MATS, bool SPLIT>
-__device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&acc)[2][4], int n, int b0, int nb, const uint32_t (&res)[4]) {
+template <int MATS, bool SPLIT, bool ADD>
+__device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&acc)[2][4], int n, int b0, int nb, const TsRes<ADD> (&res)[4]) {
     const bool bf = SPLIT && p.bf16;
     const float fmax_act = bf ? 3.3895313892515355e38f : 65504.0f;
 #pragma unroll
@@ -328,11 +332,11 @@ __device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&a
         const float cs = SPLIT && p.col_scale != nullptr ? p.col_scale[b] : 1.0f;
         if (MATS == 1) {
             float v = fminf(fmaxf((acc[0][j] + acc[1][j]) * cs, -fmax_act), fmax_act);
-            if (p.add32 != nullptr) {
-                v = __uint_as_float(res[j]) + v;
+            if constexpr (ADD) {
+                v = res[j] + v;
             } else {
                 v = ts_round(bf, v);
-                if (p.residual != nullptr) v = ts_float(bf, (uint16_t)res[j]) + v;
+                if (p.residual != nullptr) v = ts_float(bf, res[j]) + v;
             }
             p.y[o] = ts_bits(bf, v);
         } else {
@@ -349,7 +353,8 @@ __device__ __forceinline__ void ts_store_cols(const TsParams& p, const float (&a
 // SPLIT: weights in two fp16 terms, w = hi + lo with hi = (q - rint(z)) * s rounded and lo = what the rounding left out + (rint(z) - z) * s (see
 // qgemm_ts for whom).  A chunk then holds 64 k: hi in its first 32 columns, lo in the others, both multiplied with the same
 // activations.  14336 x 4096 q4, 32 bf16 rows: 26.4 us against 18.2 with one term and 93.8 of the mma.sync kernel.
-template <int BITS, int LOGG, int MATS, bool META, bool SPLIT>
+// ADD: fp32 rows are added before the rounding (a template parameter, like the modes of the mma.sync kernels, for the calls without).
+template <int BITS, int LOGG, int MATS, bool META, bool SPLIT, bool ADD>
 __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_constant__ TsParams p) {
     constexpr int KS = kRowBytes * 8 / BITS;           // k per stage: 256 (q4) or 128 (q8)
     constexpr int CK = chunk_k(SPLIT);                 // k per chunk
@@ -712,20 +717,20 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
             if (p.split == 1) {
                 if (it == 0) pdl_wait();
                 const int n = n0 + r, c0 = col_of(it) + grp * 4;
-                uint32_t res[4];
-                ts_load_residual<MATS>(p, n, c0, p.B - c0, res);
+                TsRes<ADD> res[4];
+                ts_load_residual<MATS, ADD>(p, n, c0, p.B - c0, res);
                 wait_bar(d_full, (uint32_t)it & 1u, EV_GEMV_FULL_WAIT, ok);
                 tc_fence_after();
 #pragma unroll 1
                 for (int cs = 0; cs < ncols; cs += 16) {
                     const int nb = p.B - c0 - cs;              // may be more than 4
                     if (nb <= 0) break;
-                    uint32_t next[4];
-                    ts_load_residual<MATS>(p, n, c0 + cs + 16, cs + 16 < ncols ? nb - 16 : 0, next);
+                    TsRes<ADD> next[4];
+                    ts_load_residual<MATS, ADD>(p, n, c0 + cs + 16, cs + 16 < ncols ? nb - 16 : 0, next);
                     float acc[2][4] = {};
                     tc_ld4(lane_addr + (uint32_t)(cs + grp * 4), acc[0]);
                     if (MATS == 2 || second) tc_ld4(lane_addr + (uint32_t)(ncols + cs + grp * 4), acc[1]);
-                    if (n < p.N) ts_store_cols<MATS, SPLIT>(p, acc, n, c0 + cs, nb, res);
+                    if (n < p.N) ts_store_cols<MATS, SPLIT, ADD>(p, acc, n, c0 + cs, nb, res);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) res[j] = next[j];
                 }
@@ -779,13 +784,13 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
             pdl_wait();
             const int n = row_of(0) + r;
             const float* red = reinterpret_cast<const float*>(sbase + (red_base - base));
-            uint32_t res[4];
-            ts_load_residual<MATS>(p, n, c0 + grp * 4, bcols - grp * 4, res);
+            TsRes<ADD> res[4];
+            ts_load_residual<MATS, ADD>(p, n, c0 + grp * 4, bcols - grp * 4, res);
             if (fast) wait_bar_cluster(red_bar, 0u, ok ? kTsWaitLimit : 64u);
 #pragma unroll 1
             for (int cs = grp * 4; cs < bcols; cs += 16) {
-                uint32_t next[4];
-                ts_load_residual<MATS>(p, n, c0 + cs + 16, bcols - cs - 16, next);
+                TsRes<ADD> next[4];
+                ts_load_residual<MATS, ADD>(p, n, c0 + cs + 16, bcols - cs - 16, next);
                 float acc[2][4] = {};
                 tc_ld4(lane_addr + (uint32_t)cs, acc[0]);
                 if (MATS == 2 || second) tc_ld4(lane_addr + (uint32_t)(ncols + cs), acc[1]);
@@ -799,7 +804,7 @@ __global__ void __launch_bounds__(kTsThreads, 1) qgemm_ts_kernel(const __grid_co
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             if (cs + j < bcols) acc[m][j] += red[((((q - 1) * MATS + m) * rcols + cs + j) * kRows + r)];
-                if (n < p.N) ts_store_cols<MATS, SPLIT>(p, acc, n, c0 + cs, bcols - cs, res);
+                if (n < p.N) ts_store_cols<MATS, SPLIT, ADD>(p, acc, n, c0 + cs, bcols - cs, res);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) res[j] = next[j];
             }
@@ -884,7 +889,7 @@ int max_clusters(Kernel kernel, int size, uint32_t smem) {
     return n;
 }
 
-template <int BITS, int LOGG, int MATS, bool META, bool SPLIT>
+template <int BITS, int LOGG, int MATS, bool META, bool SPLIT, bool ADD>
 int launch_ts(TsParams& p, int K, cudaStream_t stream) {
     constexpr int KS = kRowBytes * 8 / BITS;
     constexpr int CK = chunk_k(SPLIT), SC = KS / CK;
@@ -894,7 +899,7 @@ int launch_ts(TsParams& p, int K, cudaStream_t stream) {
     const int tiles = (p.N + kRows - 1) / kRows;
     p.n_stage_total = (K + KS - 1) / KS;
     p.stage_bytes = MATS * kWTile;
-    auto kernel = qgemm_ts_kernel<BITS, LOGG, MATS, META, SPLIT>;
+    auto kernel = qgemm_ts_kernel<BITS, LOGG, MATS, META, SPLIT, ADD>;
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1009,14 +1014,15 @@ int launch_ts(TsParams& p, int K, cudaStream_t stream) {
     return finish_launch();
 }
 
-template <int BITS, int LOGG, int MATS>
+template <int BITS, int LOGG, int MATS, bool ADD>
 int dispatch_ts_form(TsParams& p, int K, bool meta, bool split, cudaStream_t stream) {
-    if (!meta) return launch_ts<BITS, LOGG, MATS, false, true>(p, K, stream);
-    return split ? launch_ts<BITS, LOGG, MATS, true, true>(p, K, stream) : launch_ts<BITS, LOGG, MATS, true, false>(p, K, stream);
+    if (!meta) return launch_ts<BITS, LOGG, MATS, false, true, ADD>(p, K, stream);
+    return split ? launch_ts<BITS, LOGG, MATS, true, true, ADD>(p, K, stream) : launch_ts<BITS, LOGG, MATS, true, false, ADD>(p, K, stream);
 }
 template <int BITS, int LOGG>
 int dispatch_ts_mats(TsParams& p, int K, bool gate_up, bool meta, bool split, cudaStream_t stream) {
-    return gate_up ? dispatch_ts_form<BITS, LOGG, 2>(p, K, meta, split, stream) : dispatch_ts_form<BITS, LOGG, 1>(p, K, meta, split, stream);
+    if (gate_up) return dispatch_ts_form<BITS, LOGG, 2, false>(p, K, meta, split, stream);
+    return p.add32 != nullptr ? dispatch_ts_form<BITS, LOGG, 1, true>(p, K, meta, split, stream) : dispatch_ts_form<BITS, LOGG, 1, false>(p, K, meta, split, stream);
 }
 template <int BITS>
 int dispatch_ts(TsParams& p, int K, int G, bool gate_up, bool meta, bool split, cudaStream_t stream) {
