@@ -139,8 +139,7 @@ int b200q_gate_up_swiglu(int bits, const void* x, const uint8_t* gate_codes, con
  * out[t] = cast(y[t] + scaling[l] * B[l] (A[l] x[t])) with l = ids[t]; ids[t] < 0: out[t] = y[t].  x [rows, K], y and out [rows, N] (out
  * may be y, and y NULL: 0), A [L, R, K] and B [L, N, R], all in `dtype`; scaling [L] fp32 (NULL: 1);
  * ranks [L] (NULL: R): adapter l uses the first ranks[l] rows of A[l] and columns of B[l], the rest is not read.  fp32 sums, and one rounding
- * after the sum with y.  An id >= L counts as none and records event 10.  The factors, scaling, ranks and ids may be read before the
- * previous kernel of the stream has ended when that is a kernel of this library: none of them writes to such arrays.
+ * after the sum with y.  An id >= L counts as none and records event 10.
  * workspace: b200q_lora_workspace_bytes(rows, R) bytes of device scratch. */
 size_t b200q_lora_workspace_bytes(int64_t rows, int R);
 /* The adapters beside b200q_qmatvec: y[t] = cast(residual[t] + scaling[l] * B[l] (A[l] x[t]) + W x[t]), every sum in fp32 and one rounding

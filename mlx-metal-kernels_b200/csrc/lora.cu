@@ -45,12 +45,12 @@ struct LoraParams {
     int L, R, out32;
 };
 
-// Adapter of a row, or -1.
+// Adapter of a row, or -1.  (Both past the L1: the cluster kernel also reads them while the kernel before may still write them.)
 __device__ __forceinline__ int adapter_of(const LoraParams& p, int64_t row) {
-    const int id = p.ids[row];
+    const int id = __ldcg(p.ids + row);
     return id < p.L ? id : -1;
 }
-__device__ __forceinline__ int rank_of(const LoraParams& p, int id) { return p.ranks ? max(0, min(p.R, p.ranks[id])) : p.R; }
+__device__ __forceinline__ int rank_of(const LoraParams& p, int id) { return p.ranks ? max(0, min(p.R, __ldcg(p.ranks + id))) : p.R; }
 
 // ---- any size: a warp per value between the factors, then a thread per result ------------------------------------------------
 template <typename T> __global__ void __launch_bounds__(256) lora_shrink_any_kernel(const __grid_constant__ LoraParams p) {
@@ -203,34 +203,60 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
     const int64_t strips = (p.N + 31) / 32;
     pdl_launch_dependents();
 
-    // ---- the window's groups: every sixteenth row of an adapter leads one.  ids, ranks and factors belong to no kernel that may
-    //      still run (see the header): they are read before the wait ----
+    // ---- the window's groups: every sixteenth row of an adapter leads one ----
     const int64_t cluster = blockIdx.x / ctas, row0 = cluster / per_window * kWindow;
     const int turn = (int)(cluster % per_window);
     const bool looks = kWarps * 32 <= kWindow || threadIdx.x < kWindow;
-    const int my_id = looks && row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2;
-    if (looks) id_of[threadIdx.x] = my_id;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; my_id > -2 && i < (int)threadIdx.x / 4; ++i) {
-        const int4 v = reinterpret_cast<const int4*>(id_of)[i];
-        before += (v.x == my_id) + (v.y == my_id) + (v.z == my_id) + (v.w == my_id);
-    }
-    for (int i = threadIdx.x / 4 * 4; my_id > -2 && i < (int)threadIdx.x; ++i) before += id_of[i] == my_id;
-    if (looks) before_of[threadIdx.x] = before;
-    const unsigned lead_vote = __ballot_sync(0xFFFFFFFFu, my_id > -2 && before % kRows == 0);
-    if (lane == 0) leads[warp] = __popc(lead_vote);
-    __syncthreads();
-    int groups = 0, my_place = __popc(lead_vote & ((1u << lane) - 1u));
+    int my_id, before, groups;
+    auto read_id = [&]() { return looks && row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2; };
+    auto find_groups = [&]() {
+        if (looks) id_of[threadIdx.x] = my_id;
+        __syncthreads();
+        before = 0;
+        for (int i = 0; my_id > -2 && i < (int)threadIdx.x / 4; ++i) {
+            const int4 v = reinterpret_cast<const int4*>(id_of)[i];
+            before += (v.x == my_id) + (v.y == my_id) + (v.z == my_id) + (v.w == my_id);
+        }
+        for (int i = threadIdx.x / 4 * 4; my_id > -2 && i < (int)threadIdx.x; ++i) before += id_of[i] == my_id;
+        if (looks) before_of[threadIdx.x] = before;
+        const unsigned lead_vote = __ballot_sync(0xFFFFFFFFu, my_id > -2 && before % kRows == 0);
+        if (lane == 0) leads[warp] = __popc(lead_vote);
+        __syncthreads();
+        int my_place = __popc(lead_vote & ((1u << lane) - 1u));
+        groups = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-        if (i < warp) my_place += leads[i];
-        groups += leads[i];
+        for (int i = 0; i < kWarps; ++i) {
+            if (i < warp) my_place += leads[i];
+            groups += leads[i];
+        }
+        if (lead_vote >> lane & 1u) leaders[my_place] = threadIdx.x;
+        __syncthreads();
+    };
+    // While the kernel before ends, the groups are found from what ids and ranks say now, and the CTA's parts of the first group's
+    // factors are brought into L2.  All of it is a guess: whatever counts is read again behind the wait.
+    my_id = read_id();
+    find_groups();
+    if (turn < groups) {
+        const int id = id_of[leaders[turn]], rank = id < 0 ? 0 : rank_of(p, id);
+        const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
+        const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
+        const int64_t lines = (c_hi - c_lo + 1) / 2;         // of two chunks
+        for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
+            const int64_t r = i / lines;
+            prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
+        }
+        const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
+        for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
+            for (int64_t i = lane; i < strip_lines; i += 32)
+                if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
     }
-    if (lead_vote >> lane & 1u) leaders[my_place] = threadIdx.x;
-    __syncthreads();
+    pdl_wait();
+    const int id_now = read_id();
+    if (__syncthreads_or(id_now != my_id)) {
+        my_id = id_now;
+        find_groups();
+    }
 
-    bool waited = false;
     for (int turn_at = turn; turn_at < groups; turn_at += per_window) {      // all CTAs of a cluster agree
         const int lead = leaders[turn_at], id = id_of[lead], ahead = before_of[lead];
         if (threadIdx.x < kRows) row_of[threadIdx.x] = -1;
@@ -239,20 +265,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         const int rank = id < 0 ? 0 : rank_of(p, id);
         const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
         const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
-        if (!waited) {
-            // the CTA's parts of both factors on their way into L2 while the previous kernel ends
-            const int64_t lines = (c_hi - c_lo + 1) / 2;     // of two chunks
-            for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
-                const int64_t r = i / lines;
-                prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
-            }
-            const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
-            for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
-                for (int64_t i = lane; i < strip_lines; i += 32)
-                    if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
-            pdl_wait();
-            waited = true;
-        }
         __syncthreads();
         if (id < 0) {
             if (cta == 0 && threadIdx.x < kRows && row_of[threadIdx.x] >= 0 && p.ids[row0 + row_of[threadIdx.x]] >= p.L)
@@ -466,7 +478,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         cluster_wait();                                      // also: no CTA overwrites its sums for the next row while another reads them
         __syncthreads();
     }
-    if (!waited) pdl_wait();                                 // a grid whose blocks all end early would hide the previous kernel from the next
 }
 
 template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
