@@ -112,7 +112,8 @@ template <typename T> int any_size(const LoraParams& p, cudaStream_t stream) {
 }
 
 // ---- the cluster kernel: K a multiple of 8, R a multiple of 4 up to 256, 16-byte aligned factors and rows ------------------------
-constexpr int kRows = 16, kMaxRank = 256, kRankBlock = 64, kMaxCtas = 16;
+constexpr int kRows = 16, kMaxRank = 256, kRankBlock = 64;
+constexpr int kGather = 16;               // CTAs whose sums are fetched at a time (8: 0.6 us longer with 16 CTAs)
 constexpr int kWindow = 256;              // rows that one group may come from
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -198,14 +199,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
     T* lo = reinterpret_cast<T*>(smem + at.lo);
     const T* y = reinterpret_cast<const T*>(p.y);
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    const int64_t chunks = (p.K + 31) / 32, per = (chunks + ctas - 1) / ctas;
-    const int64_t c_lo = min(chunks, cta * per), c_hi = min(chunks, c_lo + per);
-    const int64_t strips = (p.N + 31) / 32;
+    const int K = (int)p.K, N = (int)p.N;                    // below 2^30
+    const int chunks = (K + 31) / 32, per = (chunks + (int)ctas - 1) / (int)ctas;
+    const int c_lo = min(chunks, (int)cta * per), c_hi = min(chunks, c_lo + per);
+    const int strips = (N + 31) / 32, s_first = (int)cta * kWarps + warp, s_step = (int)ctas * kWarps;
     pdl_launch_dependents();
 
     // ---- the window's groups: every sixteenth row of an adapter leads one ----
-    const int64_t cluster = blockIdx.x / ctas, row0 = cluster / per_window * kWindow;
-    const int turn = (int)(cluster % per_window);
+    const int cluster = (int)(blockIdx.x / ctas), window = cluster / per_window, turn = cluster - window * per_window;
+    const int64_t row0 = (int64_t)window * kWindow;
     const bool looks = kWarps * 32 <= kWindow || threadIdx.x < kWindow;
     int my_id, before, groups;
     auto read_id = [&]() { return looks && row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2; };
@@ -240,15 +242,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         const int id = id_of[leaders[turn]], rank = id < 0 ? 0 : rank_of(p, id);
         const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
         const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
-        const int64_t lines = (c_hi - c_lo + 1) / 2;         // of two chunks
-        for (int64_t i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
-            const int64_t r = i / lines;
-            prefetch_l2(a + r * p.K + c_lo * 32 + (i - r * lines) * 64);
+        const int lines = (c_hi - c_lo + 1) / 2;
+        for (int i = threadIdx.x; i < rank * lines; i += kWarps * 32) {
+            const int r = i / lines;
+            prefetch_l2(a + (int64_t)r * K + c_lo * 32 + (i - r * lines) * 64);
         }
-        const int64_t strip_lines = ((int64_t)p.R * 64 + 127) / 128;
-        for (int64_t s = (int64_t)cta * kWarps + warp; rank > 0 && s < strips; s += (int64_t)ctas * kWarps)
-            for (int64_t i = lane; i < strip_lines; i += 32)
-                if (s * 32 * p.R + i * 64 < p.N * p.R) prefetch_l2(b + s * 32 * p.R + i * 64);
+        const int strip_lines = (p.R * 64 + 127) / 128;
+        for (int s = s_first; rank > 0 && s < strips; s += s_step)
+            for (int i = lane; i < strip_lines; i += 32)
+                if ((int64_t)s * 32 * p.R + i * 64 < (int64_t)N * p.R) prefetch_l2(b + (int64_t)s * 32 * p.R + i * 64);
     }
     pdl_wait();
     const int id_now = read_id();
@@ -280,17 +282,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
 
         // a round's loads of B, a lane's piece for each of four instructions: j's column n is 32 s + 8 (n / 2) + 2 j + n % 2, so that a
         // lane's results are columns 32 s + 8 q .. + 7 of rows g and g + 8
-        const int64_t s_first = (int64_t)cta * kWarps + warp, s_step = (int64_t)ctas * kWarps;
         const int first_col = (g >> 1) * 8 + (g & 1), b_next = 2 * p.R;
-        const T* b_lane = b + (s_first * 32 + first_col) * p.R + q * kPer;
+        const T* b_lane = b + (int64_t)(s_first * 32 + first_col) * p.R + q * kPer;
+        const int64_t b_step = (int64_t)s_step * 32 * p.R;
         const bool ragged = rank % kPer != 0;
-        auto load_b = [&](Piece (&w)[4], const T* from, int64_t s, int k0) {
+        auto load_b = [&](Piece (&w)[4], const T* from, int s, int k0) {
             const int k = k0 + q * kPer;
-            const bool whole = s * 32 + 32 <= p.N;
+            const bool whole = s * 32 + 32 <= N;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 w[j] = {};
-                if (k < rank && (whole || s * 32 + first_col + 2 * j < p.N)) w[j] = __ldg(reinterpret_cast<const Piece*>(from + j * b_next + k0));
+                if (k < rank && (whole || s * 32 + first_col + 2 * j < N)) w[j] = __ldg(reinterpret_cast<const Piece*>(from + j * b_next + k0));
             }
             if (ragged && k < rank && k + kPer > rank)       // values behind the rank are not the adapter's
 #pragma unroll
@@ -307,18 +309,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             float acc[NT][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-            const T* ab = a + (int64_t)(rb + g) * p.K + q * 8;
-            for (int64_t c = c_lo + warp; c < c_hi; c += kWarps * U) {
+            const T* ab = a + (int64_t)(rb + g) * K + q * 8;
+            const int64_t a_step = (int64_t)8 * K;
+            for (int c = c_lo + warp; c < c_hi; c += kWarps * U) {
                 uint4 xa[U], xb[U], w[U][NT];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int64_t k = (c + u * kWarps) * 32;
-                    const bool in = c + u * kWarps < c_hi && k + q * 8 < p.K;
+                    const int k = (c + u * kWarps) * 32;
+                    const bool in = c + u * kWarps < c_hi && k + q * 8 < K;
                     xa[u] = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
                     xb[u] = in && r1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
-                        w[u][j] = in && rb + j * 8 + g < rank ? __ldg(reinterpret_cast<const uint4*>(ab + (int64_t)j * 8 * p.K + k)) : zero;
+                        w[u][j] = in && rb + j * 8 + g < rank ? __ldg(reinterpret_cast<const uint4*>(ab + j * a_step + k)) : zero;
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -332,18 +335,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 if (j * 8 >= width) break;
-                float* dst = part + ((size_t)warp * kRows + g) * width + j * 8 + 2 * q;
-                dst[0] = acc[j][0];
-                dst[1] = acc[j][1];
-                dst[8 * width] = acc[j][2];
-                dst[8 * width + 1] = acc[j][3];
+                float* dst = part + (warp * kRows + g) * width + j * 8 + 2 * q;
+                if (r0) {
+                    dst[0] = acc[j][0];
+                    dst[1] = acc[j][1];
+                }
+                if (r1) {
+                    dst[8 * width] = acc[j][2];
+                    dst[8 * width + 1] = acc[j][3];
+                }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < kRows * width; i += kWarps * 32) {
-                float s = 0.0f;
+            for (int r = warp; r < kRows; r += kWarps) {
+                if (row_of[r] < 0) continue;
+                for (int c = lane; c < width; c += 32) {
+                    float s = 0.0f;
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) s += part[(size_t)v * kRows * width + i];
-                own[(i / width) * rank8 + rb + i % width] = s;
+                    for (int v = 0; v < kWarps; ++v) s += part[(v * kRows + r) * width + c];
+                    own[r * rank8 + rb + c] = s;
+                }
             }
             __syncthreads();
         }
@@ -357,14 +367,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < kMaxRank / 32; ++i) {
                 v[i] = 0.0f;
-                const int k = i * 32 + lane;
-                if (i * 32 < rank && used) {
-                    float u[kMaxCtas];
+                const int at_k = i * 32 + lane;
+                if (i * 32 < rank && used)
+                    for (int c0 = 0; c0 < (int)ctas; c0 += kGather) {
+                        float u[kGather];
 #pragma unroll
-                    for (int c = 0; c < kMaxCtas; ++c) u[c] = c < ctas && k < rank ? load_remote(own + r * rank8 + k, c) : 0.0f;
+                        for (int c = 0; c < kGather; ++c) u[c] = c0 + c < (int)ctas && at_k < rank ? load_remote(own + r * rank8 + at_k, c0 + c) : 0.0f;
 #pragma unroll
-                    for (int c = 0; c < kMaxCtas; ++c) v[i] += u[c];
-                }
+                        for (int c = 0; c < kGather; ++c) v[i] += u[c];
+                    }
                 top = fmaxf(top, fabsf(v[i]));
             }
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -390,21 +401,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         float f[2];
         f[0] = row_scale[g];
         f[1] = row_scale[g + 8];
-        for (int64_t s = s_first; s < strips; s += s_step, b_lane += s_step * 32 * p.R) {
-            const int64_t n = s * 32 + q * 8;
+        const int64_t at0 = (row0 + t0) * p.N + q * 8, at1 = (row0 + t1) * p.N + q * 8;
+        for (int s = s_first; s < strips; s += s_step, b_lane += b_step) {
+            const int n = s * 32 + q * 8;
             uint4 was[2] = {zero, zero};                     // y of the lane's columns
             if (y != nullptr)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int t = half ? t1 : t0;
-                    if (t < 0 || n >= p.N) continue;
-                    const T* src = y + (row0 + t) * p.N + n;
+                    if ((half ? t1 : t0) < 0 || n >= N) continue;
+                    const T* src = y + (half ? at1 : at0) + s * 32;
                     if (vector_rows) {
                         was[half] = *reinterpret_cast<const uint4*>(src);
                     } else {
                         T e[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) e[i] = n + i < p.N ? src[i] : from_f32<T>(0.0f);
+                        for (int i = 0; i < 8; ++i) e[i] = n + i < N ? src[i] : from_f32<T>(0.0f);
                         was[half] = *reinterpret_cast<const uint4*>(e);
                     }
                 }
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             do {
                 Piece next[4];
                 if (k0 + kStep < rank) load_b(next, b_lane, s, k0 + kStep);
-                else if (s + s_step < strips) load_b(next, b_lane + s_step * 32 * p.R, s + s_step, 0);
+                else if (s + s_step < strips) load_b(next, b_lane + b_step, s + s_step, 0);
                 if (k0 < rank) {
                     const int k = k0 + q * kPer;
                     const Piece h0 = *reinterpret_cast<const Piece*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const Piece*>(hi + (g + 8) * at.low_stride + k);
@@ -439,8 +450,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             } while (k0 < rank);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int t = half ? t1 : t0;
-                if (t < 0 || n >= p.N) continue;
+                if ((half ? t1 : t0) < 0 || n >= N) continue;
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = acc[i >> 1][2 * half + (i & 1)] * f[half];
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = id < 0 ? to_f32(e[i]) : v[i] + to_f32(e[i]);
                 }
-                const int64_t to = (row0 + t) * p.N + n;
+                const int64_t to = (half ? at1 : at0) + s * 32;
                 if (p.out32) {
                     float* dst = reinterpret_cast<float*>(p.out) + to;
                     if (vector_rows) {
@@ -458,7 +468,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            if (n + i < p.N) dst[i] = v[i];
+                            if (n + i < N) dst[i] = v[i];
                     }
                 } else {
                     T o[8];
@@ -470,7 +480,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            if (n + i < p.N) dst[i] = o[i];
+                            if (n + i < N) dst[i] = o[i];
                     }
                 }
             }
@@ -521,7 +531,7 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     return cudaLaunchKernelEx(&cfg, kernel, p, (int)per_window, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
 }
 bool cluster_takes(const LoraParams& p) {
-    return p.K % 8 == 0 && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;
+    return p.K % 8 == 0 && p.K < (1 << 30) && p.N < (1 << 30) && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;
 }
 
 }  // namespace

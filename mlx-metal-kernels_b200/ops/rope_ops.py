@@ -61,6 +61,8 @@ class RotaryConfig:
             raise ValueError("low_freq_factor must be positive and below high_freq_factor")
         if self.scaling == "yarn" and not 0 < self.beta_slow < self.beta_fast:
             raise ValueError("beta_slow must be positive and below beta_fast")
+        if self.scaling == "yarn" and self.theta <= 1:
+            raise ValueError(f"scaling 'yarn' needs theta > 1, got {self.theta}")
         return self
 
     def pairs(self) -> int:

@@ -76,6 +76,7 @@ def test_scalings():
     (dict(head_dim=128, scaling="yarn"), "original_length"), (dict(head_dim=128, scaling="llama3"), "original_length"),
     (dict(head_dim=128, scaling="llama3", original_length=10, low_freq_factor=4.0), "low_freq_factor"),
     (dict(head_dim=128, scaling="yarn", original_length=10, beta_slow=40.0), "beta_slow"),
+    (dict(head_dim=128, scaling="yarn", original_length=10, theta=1.0), "theta > 1"),
 ])
 def test_config_refusals(bad, match):
     with pytest.raises(ValueError, match=match):
