@@ -330,7 +330,8 @@ int b200q_head_rope(const void* q, const void* k, void* q_out, void* k_out, cons
  * to q_out [T, Hq, D]; k heads (normalised, turned) and v heads (as they are) to slot positions[t] % page_size of page
  * block_table[sequences[t], positions[t] / page_size].  sequences NULL: token t belongs to sequence t.  A negative sequence marks
  * padding: zeros in q_out, nothing else.  No two tokens may share a slot.
- *   kv_bits   4 or 8: codes and fp16 scales, quantised from the rounded values with the rule of b200q_quantize_kv;
+ *   kv_bits   4 or 8: codes and fp16 scales, quantised from the rounded values as by b200q_quantize_kv, but with the scale as a product
+ *             with 1/127 or 1/7 in fp32: a value exactly half way between two codes may take the other one;
  *             16: pages [num_pages, page_size, Hkv, D] in the rows' dtype (scales NULL, group_size ignored)
  * A position outside the table records event 6 (the head is written unturned), a sequence or position without a page event 7
  * (nothing is appended for it).  b200q_rope_kv_append is the interleaved form for one new token of every sequence. */

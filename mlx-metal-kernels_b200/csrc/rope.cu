@@ -9,7 +9,7 @@
 //
 // The append form takes the fused rows [q heads | k heads | v heads] of a projection, returns the q heads and writes the k heads
 // (normalised, rotated) and the v heads (as they are) to slot pos % P of page block_table[sequence, pos / P]: as they are, or
-// quantised from the rounded values with the cache's rule (see stack.cu).
+// quantised from the rounded values: scale = max(max|v|, 1e-8) * (1/127 | 1/7), code = clip(rint(v / scale)) + (128 | 8).
 //
 // Bound by HBM for prompts and by latency for a few tokens.  A head is taken by D/16 lanes, so that a lane has two 16-byte pieces
 // of it: pieces l and l + D/16, which are the two halves of eight pairs in the half layout over whole heads.  One head per
@@ -202,13 +202,11 @@ template <typename T> __device__ __forceinline__ float piece_values(const uint4&
     }
     return top;
 }
-// max(top, 1e-8) / (127 | 7), correctly rounded: one correction of the product with the reciprocal is enough between 1e-8 and 3e38
+// Scale of a group: max(top, 1e-8) times the rounded reciprocal of 127 or 7 - one instruction, and within a step of the quotient that the
+// page quantiser (stack.cu) takes.  The codes are the same but for values exactly half way between two (14 v an odd multiple of the maximum in
+// 4 bits), which may take the other one.
 template <int CACHE> __device__ __forceinline__ float group_scale(float top) {
-    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f, inv = 1.0f / limit;
-    const float m = fmaxf(top, 1e-8f);
-    if (!(m < 3e38f)) return __fdiv_rn(m, limit);
-    const float q = m * inv;
-    return fmaf(fmaf(-q, limit, m), inv, q);
+    return fmaxf(top, 1e-8f) * (1.0f / (CACHE == CACHE_Q8 ? 127.0f : 7.0f));
 }
 // Its codes.  rint(v / scale) with the quotient rounded as a division rounds it: the product with the correctly rounded reciprocal,
 // corrected once by its exact remainder, is the correctly rounded quotient (Markstein's theorem) wherever it is large enough to matter.
@@ -715,11 +713,10 @@ __global__ void __launch_bounds__(kAnyWarps * 32) rope_any_kernel(const __grid_c
     const int groups = (D + p.G - 1) / p.G, per_byte = CACHE == CACHE_Q4 ? 2 : 1, bytes = (D + per_byte - 1) / per_byte;
     for (int d = lane; d < D; d += 32) y[d] = to_f32(from_f32<T>(y[d]));
     __syncwarp();
-    constexpr float limit = CACHE == CACHE_Q8 ? 127.0f : 7.0f;
     auto scale_of = [&](int g) {
         float m = 0.0f;
         for (int d = g * p.G; d < min(D, (g + 1) * p.G); ++d) m = fmaxf(m, fabsf(y[d]));
-        return __fdiv_rn(fmaxf(m, 1e-8f), limit);
+        return group_scale<CACHE>(m);
     };
     for (int g = lane; g < groups; g += 32) p.scales[kind][row * groups + g] = __float2half_rn(scale_of(g));
     for (int i = lane; i < bytes; i += 32) {

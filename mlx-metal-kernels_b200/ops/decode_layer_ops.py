@@ -99,7 +99,9 @@ def norm_rope_kv_append(qkv, cos, sin, positions, paged_qkv, n_heads: int, *, se
     sequences ``sequences[t]`` (None: one token of every sequence, in order; negative: padding, whose q row is zeros) ->
     q [T, Hq, D], turned; the turned k and the v rows go, quantised, into ``paged_qkv`` (a PagedQuantizedKVCache, modified in
     place; its ``lengths`` are left to the caller).  ``q_weight`` / ``k_weight`` [D]: an RMSNorm of every q / k head in front, in the
-    same pass.  ``cos`` / ``sin`` and ``layout`` as in ``rope_ops.apply_rope``.  No two tokens may share a slot.
+    same pass.  ``cos`` / ``sin`` and ``layout`` as in ``rope_ops.apply_rope``.  No two tokens may share a slot.  Codes are those of
+    ``quantize_kv_pages``, but the group's scale is a product with 1/127 (1/7), so that a value exactly half way between two codes may take
+    the other one.
 
     A position outside the table appends the k row unturned and is reported by ``_cabi.device_status()`` (event 6); a token whose
     sequence or page does not exist appends nothing (event 7).  Nothing is read on the host, so the call can be captured."""
