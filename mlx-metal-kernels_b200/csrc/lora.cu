@@ -7,9 +7,9 @@
 // sum with y is rounded once.
 //
 // One launch for both products: a thread-block cluster per adapter and up to 16 of the rows that use it.  Rows are looked at in windows of 256,
-// in which every CTA finds the groups; the clusters of a window take them in turn.  The CTAs of a cluster cut K: every warp multiplies its pieces of the rows with the factor A on mma.sync, straight from global memory - the
-// order of the summands is free, so a lane takes 16 contiguous bytes of a row as the k indices of two instructions.  The partial sums
-// meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp and round, a
+// in which every CTA finds the groups; the clusters of a window take them in turn.  The CTAs of a cluster cut K: every warp multiplies its pieces
+// of the rows with the factor A on mma.sync, straight from global memory - the order of the summands is free, so a lane takes 16
+// contiguous bytes of a row as the k indices of two instructions.  The partial sums meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp and round, a
 // lane with contiguous bytes of B again and 16 bytes of y, the next round's loads in flight during this one's products.  The values
 // between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
 //
