@@ -7,14 +7,16 @@
 // sum with y is rounded once.
 //
 // One launch for both products: a thread-block cluster per adapter and up to 16 of the rows that use it.  Rows are looked at in windows of 256,
-// in which every CTA finds the groups; the clusters of a window take them in turn.  The CTAs of a cluster cut K: every warp multiplies its pieces
-// of the rows with the factor A on mma.sync, straight from global memory - the order of the summands is free, so a lane takes 16
-// contiguous bytes of a row as the k indices of two instructions.  The partial sums meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp and round, a
-// lane with contiguous bytes of B again and 16 bytes of y, the next round's loads in flight during this one's products.  The values
-// between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
+// in which every CTA finds the groups; the clusters of a window take them in turn, or, when there are more of them than groups, slices of a
+// group's columns.  The CTAs of a cluster cut K: every warp multiplies its pieces of the rows with the factor A on mma.sync, straight from
+// global memory - the order of the summands is free, so a lane takes 16 contiguous bytes of a row as the k indices of two instructions.
+// The partial sums meet in shared memory, then through distributed shared memory in every CTA; then the CTAs cut N: 32 columns per warp
+// and round, a lane with contiguous bytes of B again and 16 bytes of y, the next rounds' loads in flight during this one's products.  The
+// values between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
 //
-// Bound by latency for a few rows (a chain of ids, first factor, two meetings, second factor), by L2 for prompts, whose groups of 16 rows read
-// both factors again.
+// Bound by latency for a few rows (a chain of ids, first factor, two meetings, second factor: 5.9 us for one row of rank 16, 4096 x 4096, and
+// 13.5 for 32 rows of 24 adapters of rank 64, 6144 x 4096, 2.3 TB/s), by L2 and the products for prompts, whose groups of 16 rows read both factors
+// again (512 rows of rank 64, 14336 x 4096: 30 us).
 #include "common.cuh"
 
 #include <algorithm>
@@ -135,6 +137,12 @@ __device__ __forceinline__ float load_remote(const float* local, uint32_t cta) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+// 16 bytes into shared memory behind the thread's back, or zeros
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const __half*) {
@@ -163,9 +171,9 @@ __device__ __forceinline__ void keep_ranks(uint4& v, int n) {
 // shared memory: partial sums of the warps, of the CTA, and the two terms of the rows between the factors
 struct LoraSmem {
     int low_stride;           // 16-bit values per row of a term: the rank in whole steps of 32, and 8 against bank conflicts
-    size_t part, cta, hi, lo, bytes;
+    size_t part, cta, hi, lo, ring, bytes;
 };
-__host__ __device__ inline LoraSmem lora_smem(int R, int warps) {
+__host__ __device__ inline LoraSmem lora_smem(int R, int warps, int depth) {
     LoraSmem s;
     const int block = R < kRankBlock ? (R + 7) / 8 * 8 : kRankBlock;
     s.low_stride = (R + 31) / 32 * 32 + 8;
@@ -173,16 +181,22 @@ __host__ __device__ inline LoraSmem lora_smem(int R, int warps) {
     s.cta = s.part + sizeof(float) * warps * kRows * block;
     s.hi = s.cta + sizeof(float) * kRows * ((R + 7) / 8 * 8);
     s.lo = s.hi + 2 * (size_t)kRows * s.low_stride;
-    s.bytes = s.lo + 2 * (size_t)kRows * s.low_stride;
+    s.ring = s.lo + 2 * (size_t)kRows * s.low_stride;
+    s.bytes = s.ring + sizeof(uint4) * 32 * 4 * depth * warps;
     return s;
 }
 
 // NT: rank tiles of 8 that a warp accumulates at a time.  NT 2 takes ranks by 16 (8 bytes of B per lane), NT 4 and 8 by 32 (16 bytes).
-template <typename T, int NT, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __grid_constant__ LoraParams p, int per_window, int vector_rows) {
+// For these two rounds of B are in flight in a ring of shared memory, from before the products with A on (NT 2: one, in registers).  32 and 512
+// rows of rank 64, fp16, with a projection 6144 x 4096: 22.5 -> 21.5 us, 68.4 -> 66.8; three or four rounds ahead: 21.8, 22.1 and 67.2.
+constexpr int ring_depth(int NT) { return NT <= 2 ? 0 : 2; }
+// SLICED: several clusters may take slices of a group's columns (a template parameter: one row 10.9 us against 11.3 with the choice at run time).
+template <typename T, int NT, int kWarps, bool SLICED>
+__global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __grid_constant__ LoraParams p, int per_window, int max_slices, int vector_rows) {
     using Piece = std::conditional_t<NT <= 2, uint2, uint4>;
     constexpr int kPer = sizeof(Piece) / 2;                  // ranks in a lane's piece
     constexpr int kStep = 4 * kPer;                          // ranks of a round
+    constexpr int DEPTH = ring_depth(NT);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float row_scale[kRows];
     __shared__ __align__(16) int id_of[kWindow];             // -1: none, -2: no such row
@@ -192,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
     __shared__ int row_of[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const uint32_t cta = cluster_rank(), ctas = cluster_size();
-    const LoraSmem at = lora_smem(p.R, kWarps);
+    const LoraSmem at = lora_smem(p.R, kWarps, DEPTH);
     float* part = reinterpret_cast<float*>(smem + at.part);
     float* own = reinterpret_cast<float*>(smem + at.cta);
     T* hi = reinterpret_cast<T*>(smem + at.hi);
@@ -202,14 +216,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
     const int K = (int)p.K, N = (int)p.N;                    // below 2^30
     const int chunks = (K + 31) / 32, per = (chunks + (int)ctas - 1) / (int)ctas;
     const int c_lo = min(chunks, (int)cta * per), c_hi = min(chunks, c_lo + per);
-    const int strips = (N + 31) / 32, s_first = (int)cta * kWarps + warp, s_step = (int)ctas * kWarps;
+    const int strips = (N + 31) / 32;
     pdl_launch_dependents();
 
     // ---- the window's groups: every sixteenth row of an adapter leads one ----
     const int cluster = (int)(blockIdx.x / ctas), window = cluster / per_window, turn = cluster - window * per_window;
     const int64_t row0 = (int64_t)window * kWindow;
     const bool looks = kWarps * 32 <= kWindow || threadIdx.x < kWindow;
-    int my_id, before, groups;
+    int my_id, before, groups, slices;
     auto read_id = [&]() { return looks && row0 + threadIdx.x < p.rows ? max(adapter_of(p, row0 + threadIdx.x), -1) : -2; };
     auto find_groups = [&]() {
         if (looks) id_of[threadIdx.x] = my_id;
@@ -232,14 +246,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             groups += leads[i];
         }
         if (lead_vote >> lane & 1u) leaders[my_place] = threadIdx.x;
+        // fewer groups than clusters: several clusters take slices of a group's columns, and all of its products with A
+        slices = SLICED && groups > 0 && 2 * groups <= per_window ? min(per_window / groups, max_slices) : 1;
         __syncthreads();
     };
-    // While the kernel before ends, the groups are found from what ids and ranks say now, and the CTA's parts of the first group's
+    // While the kernel before ends, the groups are found from what ids and ranks say now, and the CTA's slices of the first group's
     // factors are brought into L2.  All of it is a guess: whatever counts is read again behind the wait.
     my_id = read_id();
     find_groups();
-    if (turn < groups) {
-        const int id = id_of[leaders[turn]], rank = id < 0 ? 0 : rank_of(p, id);
+    if (turn < groups * slices) {
+        const int slice = SLICED && slices > 1 ? turn / groups : 0;
+        const int id = id_of[leaders[turn - slice * groups]], rank = id < 0 ? 0 : rank_of(p, id);
         const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)max(id, 0) * p.R * p.K;
         const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.N * p.R;
         const int lines = (c_hi - c_lo + 1) / 2;
@@ -248,7 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             prefetch_l2(a + (int64_t)r * K + c_lo * 32 + (i - r * lines) * 64);
         }
         const int strip_lines = (p.R * 64 + 127) / 128;
-        for (int s = s_first; rank > 0 && s < strips; s += s_step)
+        for (int s = (slice * (int)ctas + (int)cta) * kWarps + warp; rank > 0 && s < strips; s += slices * (int)ctas * kWarps)
             for (int i = lane; i < strip_lines; i += 32)
                 if ((int64_t)s * 32 * p.R + i * 64 < (int64_t)N * p.R) prefetch_l2(b + (int64_t)s * 32 * p.R + i * 64);
     }
@@ -259,8 +276,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         find_groups();
     }
 
-    for (int turn_at = turn; turn_at < groups; turn_at += per_window) {      // all CTAs of a cluster agree
-        const int lead = leaders[turn_at], id = id_of[lead], ahead = before_of[lead];
+    for (int item = turn; item < groups * slices; item += per_window) {      // all CTAs of a cluster agree
+        const int slice = SLICED && slices > 1 ? item / groups : 0, s_first = (slice * (int)ctas + (int)cta) * kWarps + warp, s_step = slices * (int)ctas * kWarps;
+        const int lead = leaders[item - slice * groups], id = id_of[lead], ahead = before_of[lead];
         if (threadIdx.x < kRows) row_of[threadIdx.x] = -1;
         __syncthreads();
         if (my_id == id && before >= ahead && before < ahead + kRows) row_of[before - ahead] = threadIdx.x;
@@ -299,7 +317,33 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
                 for (int j = 0; j < 4; ++j) keep_ranks(w[j], rank - k);
         };
         Piece w[4];
-        if (NT <= 4) load_b(w, b_lane, s_first, 0);          // NT 8 has no registers for it yet
+        // the ring: a lane copies its pieces of the rounds ahead and reads them back itself, so that nothing but its own copies is waited for
+        uint4* ring = reinterpret_cast<uint4*>(smem + at.ring) + warp * (DEPTH * 4 * 32) + lane;
+        const T* ring_b = b_lane;
+        int ring_s = s_first, ring_k = 0, ring_at = 0;
+        auto copy_round = [&]() {                            // of the round that ring_s and ring_k are at; into the slot that was read last
+            if (ring_s < strips && rank > 0) {
+                const bool in = ring_k + q * kPer < rank;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool live = in && ring_s * 32 + first_col + 2 * j < N;
+                    cp_async16_or_zero(ring + (ring_at * 4 + j) * 32, live ? ring_b + j * b_next + ring_k : b, live);
+                }
+                ring_k += kStep;
+                if (ring_k >= rank) {
+                    ring_k = 0;
+                    ring_s += s_step;
+                    ring_b += b_step;
+                }
+            }
+            cp_async_commit();
+            if (++ring_at == DEPTH) ring_at = 0;
+        };
+        if constexpr (DEPTH > 0) {
+            for (int i = 0; i < DEPTH; ++i) copy_round();
+        } else {
+            load_b(w, b_lane, s_first, 0);
+        }
 
         // ---- rows times A: the CTA's chunks of 32 k, dealt to its warps; a lane holds k = 8q .. 8q + 7 of a chunk ----
         const T* x0 = reinterpret_cast<const T*>(p.x) + (row0 + max(t0, 0)) * p.K + q * 8;
@@ -359,7 +403,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
         }
         // ---- the CTAs' sums meet in every CTA: a warp per row, as two terms and a power of two ----
         cluster_arrive();
-        if (NT > 4) load_b(w, b_lane, s_first, 0);
         cluster_wait();
         for (int r = warp; r < kRows; r += kWarps) {
             const bool used = row_of[r] >= 0;
@@ -425,8 +468,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
             int k0 = 0;
             do {
                 Piece next[4];
-                if (k0 + kStep < rank) load_b(next, b_lane, s, k0 + kStep);
-                else if (s + s_step < strips) load_b(next, b_lane + b_step, s + s_step, 0);
+                if constexpr (DEPTH > 0) {
+                    if (k0 < rank) {
+                        cp_async_wait<DEPTH - 1>();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const Piece*>(ring + (ring_at * 4 + j) * 32);
+                        const int k = k0 + q * kPer;
+                        if (ragged && k < rank && k + kPer > rank)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) keep_ranks(w[j], rank - k);
+                    }
+                } else {
+                    if (k0 + kStep < rank) load_b(next, b_lane, s, k0 + kStep);
+                    else if (s + s_step < strips) load_b(next, b_lane + b_step, s + s_step, 0);
+                }
                 if (k0 < rank) {
                     const int k = k0 + q * kPer;
                     const Piece h0 = *reinterpret_cast<const Piece*>(hi + g * at.low_stride + k), h1 = *reinterpret_cast<const Piece*>(hi + (g + 8) * at.low_stride + k);
@@ -444,8 +499,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
                         }
                     }
                 }
+                if constexpr (DEPTH > 0) {
+                    if (k0 < rank) copy_round();             // behind the products: the slot has been read
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = next[j];
+                    for (int j = 0; j < 4; ++j) w[j] = next[j];
+                }
                 k0 += kStep;
             } while (k0 < rank);
 #pragma unroll
@@ -493,13 +552,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_cluster_kernel(const __gr
 template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream) {
     const bool narrow = p.R <= 16 || p.R % 8 != 0 || ((uintptr_t)p.b & 15u) != 0, wide = !narrow && p.R > 32;
     const int64_t windows = (p.rows + kWindow - 1) / kWindow, slots = (int64_t)sm_count() * 2;
-    // CTAs per cluster.  As many as leave every row a cluster of its own on the GPU at once; four at least, or eight where a group reads a MB
-    // of factors - there are hardly as many adapters as rows - but fewer when the groups of 16 rows alone fill the GPU.  With the
-    // projection, us for 4 / 8 / 16: one row, rank 16, 4096 x 4096: 12.3 / 10.5 / 9.9; 32 rows, rank 64, 6144 x 4096: 37.5 / 31.3 / 37.1; 128 rows of 32
-    // adapters, rank 16: 22.2 / 25.6 / 33.3; 512 rows, rank 64, 14336 x 4096: 127 / 120 / 132.
+    // CTAs per cluster.  As many as leave every row a cluster of its own on the GPU at once; four at least (eight where a group reads a MB of
+    // factors, and the rows fill no window, or 4 MB: few groups then) but fewer when the groups of 16 rows alone fill the GPU.  With
+    // the projection, us for 4 / 8 / 16: one row, rank 16, 4096 x 4096: 12.2 / 11.0 / 10.7; 32 rows, rank 64, 6144 x 4096: 33.7 / 29.1 / 35.5; 128 rows of 32
+    // adapters, rank 16, 4096 x 4096: 24.0 / 26.9 / 36.7; 512 rows, rank 64, 14336 x 4096: 113.3 / 121.0 / 133; 64 rows of 8 adapters of rank 64, 6144 x
+    // 4096: 26.3 / 23.9, 512: 61.8 / 66.6; of rank 256, 512 rows: 104.5 / 96.9.
     int ctas = tuning_get("lora.cluster");
     if (ctas <= 0) {
-        const int least = (int64_t)p.R * (p.K + p.N) >= 512 * 1024 ? 8 : 4;
+        const int64_t factors = (int64_t)p.R * (p.K + p.N);      // values that a group reads
+        const int least = factors >= 2048 * 1024 || (factors >= 512 * 1024 && p.rows < kWindow) ? 8 : 4;
         ctas = 16;
         while (ctas > least && p.rows * ctas > slots) ctas /= 2;
         while (ctas > 1 && (p.rows + kRows - 1) / kRows * ctas > slots) ctas /= 2;
@@ -507,10 +568,17 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     // clusters per window: one for each of its rows, as far as the GPU holds them
     const int64_t rows = std::min<int64_t>(p.rows, kWindow), per_window = std::min(rows, std::max<int64_t>(1, slots / ctas / windows));
     const int64_t clusters = windows * per_window;
+    // clusters per group at most, when there are more of them than groups: each warp keeps two rounds of B or more (with projections of 6144 x 4096:
+    // 128 rows of one adapter of rank 64 34.3 -> 32.0 us, of eight adapters of rank 256 71.1 -> 59.0; one round: 32 rows of 8 adapters of rank 32 17.7 -> 18.8)
+    const int64_t turns = ((p.N + 31) / 32 + ctas * 8 - 1) / (ctas * 8), rounds = turns * ((p.R + (narrow ? 15 : 31)) / (narrow ? 16 : 32));
+    const int max_slices = (int)std::max<int64_t>(1, std::min(turns, rounds / 2));
     if (clusters > INT32_MAX / ctas) return B200Q_ERR_UNSUPPORTED;
     const int warps = 8;
-    const size_t smem = lora_smem(p.R, warps).bytes;
-    void (*kernel)(const LoraParams, int, int) = narrow ? lora_cluster_kernel<T, 2, 8> : wide ? lora_cluster_kernel<T, 8, 8> : lora_cluster_kernel<T, 4, 8>;
+    const size_t smem = lora_smem(p.R, warps, ring_depth(narrow ? 2 : 8)).bytes;
+    const bool sliced = max_slices > 1 && 2 * ((rows + kRows - 1) / kRows) <= per_window;      // there can be clusters enough
+    void (*kernel)(const LoraParams, int, int, int) =
+        sliced ? (narrow ? lora_cluster_kernel<T, 2, 8, true> : wide ? lora_cluster_kernel<T, 8, 8, true> : lora_cluster_kernel<T, 4, 8, true>)
+               : (narrow ? lora_cluster_kernel<T, 2, 8, false> : wide ? lora_cluster_kernel<T, 8, 8, false> : lora_cluster_kernel<T, 4, 8, false>);
     if (smem > 40 * 1024 &&      // with the static part beyond what needs no asking
          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
     if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return B200Q_ERR_LAUNCH;
@@ -528,7 +596,7 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     cfg.attrs = attr;
     cfg.numAttrs = tuning_get("no_pdl") ? 1 : 2;
     const int vector_rows = p.N % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) & 15u) == 0;      // results in 16-byte pieces
-    return cudaLaunchKernelEx(&cfg, kernel, p, (int)per_window, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, p, (int)per_window, max_slices, vector_rows) == cudaSuccess ? finish_launch() : B200Q_ERR_LAUNCH;
 }
 bool cluster_takes(const LoraParams& p) {
     return p.K % 8 == 0 && p.K < (1 << 30) && p.N < (1 << 30) && p.R % 4 == 0 && p.R <= kMaxRank && (((uintptr_t)p.x | (uintptr_t)p.a) & 15u) == 0 && ((uintptr_t)p.b & 7u) == 0;

@@ -76,6 +76,15 @@ def test_lora_add(cuda, rows, N, K, L, R, dtype, spread):
     assert cabi.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,N,K,L,R", [(8, 6144, 96, 1, 40), (32, 6144, 256, 1, 64), (32, 6149, 64, 2, 64), (40, 6144, 64, 1, 24),
+                                          (128, 4100, 128, 3, 256), (200, 8200, 64, 2, 16), (270, 8192, 40, 1, 128)])
+@pytest.mark.parametrize("spread", ["mixed", "runs"])
+def test_many_rows_of_few_adapters(cuda, rows, N, K, L, R, dtype, spread):
+    """Fewer groups of rows than clusters: several share a group's columns."""
+    test_lora_add(cuda, rows, N, K, L, R, dtype, spread)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("rows,N,K,G", [(1, 512, 1024, 64), (6, 1003, 96, 32), (40, 256, 512, 64)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
