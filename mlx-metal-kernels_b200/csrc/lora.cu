@@ -15,7 +15,7 @@
 // values between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
 //
 // Bound by latency for a few rows (a chain of ids, first factor, two meetings, second factor: 5.9 us for one row of rank 16, 4096 x 4096, and
-// 13.5 for 32 rows of 24 adapters of rank 64, 6144 x 4096, 2.3 TB/s), by L2 and the products for prompts, whose groups of 16 rows read both factors
+// 13.5 for 32 rows of 24 adapters of rank 64, 6144 x 4096, 1.8 TB/s), by L2 and the products for prompts, whose groups of 16 rows read both factors
 // again (512 rows of rank 64, 14336 x 4096: 30 us).
 #include "common.cuh"
 
