@@ -313,6 +313,19 @@ def test_large_pools(cuda):
     w.compact()
 
 
+def test_long_lists(cuda):
+    """More sequences, children and pages in a call than the plans have threads, and padding in between."""
+    B = 2600
+    w = World(cuda, "bytes", 1, 4500, 3, B, 4, seed=8)
+    assert w.grow([4] * 1300 + [0] * 1300) == 0
+    children = [-1 if i % 7 == 0 else 1300 + i for i in range(1300)]
+    assert w.fork(list(range(1300)), children) == 0
+    assert w.copy(list(range(1500)), list(range(2999, 1499, -1))) == 0
+    assert w.copy(list(range(1500)), list(range(2998, 1498, -1))) == 8
+    w.release([b for b in range(B) if b % 3] * 2)
+    w.compact()
+
+
 def test_offsets_past_32_bits(cuda):
     """Pages behind the first 4 GB of a tensor."""
     n, shape = 280000, (16, 8, 128)

@@ -214,3 +214,37 @@ def test_streams_and_graphs(cuda):
     for graph in graphs + graphs:
         graph.replay()
     assert torch.equal(outs[0], fresh) and torch.equal(outs[1], fresh) and not torch.equal(fresh, want)
+
+
+@pytest.mark.parametrize("R,ranks", [(24, (13, 0, 8)), (64, (33, 5, 64)), (136, (71, 1, 130))])
+@pytest.mark.parametrize("N,rows", [(6144, 12), (200, 40)])
+def test_values_behind_the_ranks_of_wide_factors(cuda, R, ranks, N, rows):
+    """What lies behind an adapter's rank, NaN here, stays out of the products, wherever the rank ends in a piece of eight."""
+    K = 96
+    ad = make(3, R, K, N, torch.bfloat16, cuda, R, list(ranks))
+    x = torch.randn((rows, K), generator=gen(21)).to(torch.bfloat16).to(cuda)
+    y = torch.randn((rows, N), generator=gen(22)).to(torch.bfloat16).to(cuda)
+    ids = (torch.arange(rows, dtype=torch.int32, device=cuda) % 4) - 1
+    clean = lora.lora_add(y, x, ad, ids)
+    check(clean, y, x, ad, ids)
+    for l, rank in enumerate(ranks):
+        ad.a[l, rank:] = float("nan")
+        ad.b[l, :, rank:] = float("nan")
+    assert torch.equal(lora.lora_add(y, x, ad, ids), clean)
+
+
+@pytest.mark.parametrize("K,R", [(64, 8), (63, 8)])
+def test_thousands_of_rows_and_results_in_place(cuda, K, R):
+    """Many windows of rows, one CTA per cluster; the C call with out = y."""
+    rows, N, L = 5000, 72, 6
+    ad = make(L, R, K, N, torch.float16, cuda, 31)
+    x = torch.randn((rows, K), generator=gen(32)).half().to(cuda)
+    y = torch.randn((rows, N), generator=gen(33)).half().to(cuda)
+    ids = torch.randint(-1, L, (rows,), generator=gen(34), dtype=torch.int32).to(cuda)
+    got = lora.lora_add(y, x, ad, ids)
+    check(got, y, x, ad, ids)
+    lib = cabi.load()
+    ws = torch.empty(lib.b200q_lora_workspace_bytes(rows, R), dtype=torch.uint8, device=cuda)
+    cabi.check(lib.b200q_lora_add(x.data_ptr(), y.data_ptr(), y.data_ptr(), ad.a.data_ptr(), ad.b.data_ptr(), ad.scaling.data_ptr(), None,
+                                  ids.data_ptr(), rows, N, K, L, R, cabi.F16, ws.data_ptr(), ws.numel(), cabi.stream()), "b200q_lora_add")
+    assert torch.equal(y, got)

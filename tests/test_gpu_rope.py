@@ -463,3 +463,39 @@ def test_append_of_many_tokens(cuda, bits, D, R, G, layout):
         page, slot = table[seq.clamp(0, B - 1).long(), (pos // P).long()].long(), (pos % P).long()
         held = (seq >= 0) & (seq < B) & (page >= 0)
         assert_quantisers_agree(results[0][2][page[held], slot[held]], results[0][4][page[held], slot[held]], v[held], bits, G)
+
+
+def test_captured_calls_of_many_tokens(cuda):
+    """Two graphs over the ring kernel, replayed in turn on rows, positions and sequences that were not there at capture."""
+    T, P, Hq, Hkv, D, B = many(cuda), 16, 4, 2, 128, 3
+    blocks = T // B // P + 3
+    table = torch.randperm(B * blocks, generator=gen(41)).to(torch.int32).reshape(B, blocks).to(cuda)
+    cos, sin = (t.to(cuda) for t in tables(D, blocks * P))
+    w = (1 + 0.1 * torch.randn(D, generator=gen(42))).to(torch.bfloat16).to(cuda)
+    pools = [torch.zeros((B * blocks, P, Hkv, D), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    qkv = torch.randn((T, (Hq + 2 * Hkv) * D), generator=gen(43)).to(torch.bfloat16).to(cuda)
+    seq = (torch.arange(T, dtype=torch.int32) % B).to(cuda)
+    pos = (torch.arange(T, dtype=torch.int32) // B).to(cuda)
+    calls = (lambda: pkv_ops.norm_rope_kv_append_pages(qkv, cos, sin, pos, *pools, table, Hq, sequences=seq, q_weight=w, k_weight=w),
+             lambda: rope_ops.apply_rope(qkv.view(T, -1, D)[:, :Hq], None, cos, sin, pos)[0])
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call())
+    qkv.copy_(torch.randn(qkv.shape, generator=gen(44)))
+    pos.copy_(pos.flip(0).clone())
+    seq.copy_(seq.flip(0).clone())
+    seq[5::40] = -1
+    for p in pools:
+        p.zero_()
+    for graph in graphs + graphs:
+        graph.replay()
+    replayed = [p.clone() for p in pools]
+    for p in pools:
+        p.zero_()
+    assert all(torch.equal(out, call()) for out, call in zip(outs, calls)) and all(torch.equal(a, b) for a, b in zip(replayed, pools))
+    assert bool((outs[0][5::40] == 0).all()) and cabi.device_status() == 0
