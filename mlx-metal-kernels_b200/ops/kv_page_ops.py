@@ -13,6 +13,7 @@ padding, so that a captured call can serve fewer sequences than it was captured 
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass
 from typing import Any
 
@@ -136,7 +137,7 @@ def reserve_pages(pool: PagePool, block_table, lengths, new_tokens) -> None:
         if per_row.shape[0] != B:
             raise ValueError(f"new_tokens must have shape {(B,)}, got {tuple(per_row.shape)}")
     else:
-        uniform = int(new_tokens)
+        uniform = operator.index(new_tokens)
         if not 0 <= uniform < 2 ** 31:
             raise ValueError(f"new_tokens must be in [0, 2^31), got {new_tokens}")
     device = _cabi.require_cuda(pool.ref_counts, block_table, lengths, per_row)

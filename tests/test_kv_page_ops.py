@@ -124,3 +124,9 @@ def test_c_abi_refuses_bad_arguments():
     args = list(cases["b200q_reserve_pages"][0])
     args[7] = (1 << 24) + 1
     assert lib.b200q_reserve_pages(*args) == -2
+
+
+def test_fractions_of_tokens():
+    pool, table, lengths = setup()
+    with pytest.raises(TypeError):
+        pages.reserve_pages(pool, table, lengths, 1.5)
