@@ -140,7 +140,7 @@ int b200q_gate_up_swiglu(int bits, const void* x, const uint8_t* gate_codes, con
  * may be y, and y NULL: 0), A [L, R, K] and B [L, N, R], all in `dtype`; scaling [L] fp32 (NULL: 1);
  * ranks [L] (NULL: R): adapter l uses the first ranks[l] rows of A[l] and columns of B[l], the rest is not read.  fp32 sums, and one rounding
  * after the sum with y.  An id >= L counts as none and records event 10.
- * workspace: b200q_lora_workspace_bytes(rows, R) bytes of device scratch. */
+ * workspace: b200q_lora_workspace_bytes(rows, R) bytes of device scratch, 16-byte aligned (as that of b200q_lora_qmatvec). */
 size_t b200q_lora_workspace_bytes(int64_t rows, int R);
 /* The adapters beside b200q_qmatvec: y[t] = cast(residual[t] + scaling[l] * B[l] (A[l] x[t]) + W x[t]), every sum in fp32 and one rounding
  * (residual may be NULL).  Arguments as in b200q_qmatvec and b200q_lora_add; the matvec takes what b200q_scratch_next left for it. */

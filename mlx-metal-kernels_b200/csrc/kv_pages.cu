@@ -502,7 +502,7 @@ int reserve_pages_impl(int32_t* refs, int64_t num_pages, int32_t* table, const i
     if (num_pages <= 0 || num_pages > INT32_MAX || B <= 0 || max_blocks <= 0 || page_size <= 0 || (new_tokens == nullptr && uniform < 0))
         return B200Q_ERR_BAD_ARG;
     if (max_blocks > kMaxBlocks) return B200Q_ERR_UNSUPPORTED;
-    if (ws == nullptr || ws_bytes < reserve_workspace_impl(B, num_pages)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < reserve_workspace_impl(B, num_pages)) return B200Q_ERR_WORKSPACE;
     int32_t* need_row = (int32_t*)ws;
     return launch(stream, 1, kPlanThreads, reserve_kernel, refs, num_pages, table, lengths, new_tokens, uniform, B, max_blocks, page_size,
                   need_row, need_row + num_pages, num_pages, need_row + 2 * num_pages);
@@ -519,7 +519,7 @@ int copy_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* bas
                     const int32_t* dst, int n, int64_t num_pages, int page_size, void* ws, size_t ws_bytes, cudaStream_t stream) {
     if (bad_tensors(bases0, n0, slot0, bases1, n1, slot1) || src == nullptr || dst == nullptr) return B200Q_ERR_BAD_ARG;
     if (num_pages <= 0 || num_pages > INT32_MAX || n <= 0 || page_size <= 0) return B200Q_ERR_BAD_ARG;
-    if (ws == nullptr || ws_bytes < copy_workspace_impl(n, num_pages)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < copy_workspace_impl(n, num_pages)) return B200Q_ERR_WORKSPACE;
     Header* header = (Header*)ws;
     Move* moves = (Move*)(header + 1);
     const int rc = launch(stream, 1, kPlanThreads, copy_plan_kernel, src, dst, n, num_pages, page_size, header, moves, (int32_t*)(moves + n));
@@ -533,7 +533,7 @@ int fork_sequences_impl(void* const* bases0, int n0, int64_t slot0, void* const*
         children == nullptr)
         return B200Q_ERR_BAD_ARG;
     if (num_pages <= 0 || num_pages > INT32_MAX || n <= 0 || B <= 0 || max_blocks <= 0 || page_size <= 0) return B200Q_ERR_BAD_ARG;
-    if (ws == nullptr || ws_bytes < fork_workspace_impl(n, B)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < fork_workspace_impl(n, B)) return B200Q_ERR_WORKSPACE;
     Header* header = (Header*)ws;
     Move* moves = (Move*)(header + 1);
     const int rc = launch(stream, 1, kPlanThreads, fork_plan_kernel, refs, num_pages, table, lengths, parents, children, n, B, max_blocks,
@@ -548,7 +548,7 @@ int compact_pages_impl(void* const* bases0, int n0, int64_t slot0, void* const* 
                        cudaStream_t stream) {
     if (bad_tensors(bases0, n0, slot0, bases1, n1, slot1) || refs == nullptr || table == nullptr || remap == nullptr) return B200Q_ERR_BAD_ARG;
     if (num_pages <= 0 || num_pages > INT32_MAX || B <= 0 || max_blocks <= 0 || page_size <= 0) return B200Q_ERR_BAD_ARG;
-    if (ws == nullptr || ws_bytes < compact_workspace_impl(num_pages)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < compact_workspace_impl(num_pages)) return B200Q_ERR_WORKSPACE;
     Header* header = (Header*)ws;
     Move* moves = (Move*)(header + 1);
     const int rc = launch(stream, 1, kPlanThreads, compact_plan_kernel, refs, num_pages, page_size, header, moves, remap);

@@ -617,7 +617,7 @@ int lora_add_impl(const void* x, const void* y, void* out, const void* a, const 
                   cudaStream_t stream) {
     if (x == nullptr || out == nullptr || a == nullptr || b == nullptr || ids == nullptr) return B200Q_ERR_BAD_ARG;
     if (rows <= 0 || N <= 0 || K <= 0 || L <= 0 || R <= 0 || !is_act_dtype(dtype)) return B200Q_ERR_BAD_ARG;
-    if (ws == nullptr || ws_bytes < lora_workspace_impl(rows, R)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < lora_workspace_impl(rows, R)) return B200Q_ERR_WORKSPACE;
     return lora_rows({x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R, 0}, dtype, ws_bytes, stream);
 }
 
@@ -634,7 +634,7 @@ int lora_qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void*
         !is_scale_dtype(scale_dtype))
         return B200Q_ERR_BAD_ARG;
     if (N > INT32_MAX || K > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
-    if (ws == nullptr || ws_bytes < lora_qmatvec_workspace_impl(rows, N, R)) return B200Q_ERR_WORKSPACE;
+    if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < lora_qmatvec_workspace_impl(rows, N, R)) return B200Q_ERR_WORKSPACE;
     const size_t low = low_rows_bytes(rows, N);
     const int rc = lora_rows({x, residual, ws, a, b, scaling, ranks, ids, (float*)((uint8_t*)ws + low), rows, K, N, L, R, 1}, act_dtype, ws_bytes - low, stream);
     if (rc != B200Q_OK) return rc;

@@ -130,3 +130,12 @@ def test_fractions_of_tokens():
     pool, table, lengths = setup()
     with pytest.raises(TypeError):
         pages.reserve_pages(pool, table, lengths, 1.5)
+
+
+def test_c_abi_refuses_workspaces_that_are_not_aligned():
+    lib = cabi.load()
+    one = (ctypes.c_void_p * 2)(16, 16)
+    assert lib.b200q_reserve_pages(16, 8, 16, 16, None, 1, 3, 2, 4, 20, 1 << 20, None) == -4
+    assert lib.b200q_copy_pages(one, 2, 64, None, 0, 0, 16, 16, 1, 8, 4, 20, 1 << 20, None) == -4
+    assert lib.b200q_fork_sequences(one, 2, 64, one, 2, 8, 16, 8, 16, 16, 16, 16, 1, 3, 2, 4, 20, 1 << 20, None) == -4
+    assert lib.b200q_compact_pages(one, 2, 64, one, 2, 8, 16, 8, 16, 3, 2, 4, 16, 20, 1 << 20, None) == -4

@@ -98,3 +98,9 @@ def test_c_abi_refuses_bad_arguments():
         args[i] = 2 ** 31
         assert lib.b200q_lora_qmatvec(*args) == -2
     assert lib.b200q_lora_qmatvec_workspace_bytes(2, 32, 4) >= 2 * 32 * 4 + 32 and lib.b200q_lora_qmatvec_workspace_bytes(0, 32, 4) == 0
+
+
+def test_c_abi_refuses_workspaces_that_are_not_aligned():
+    lib = cabi.load()
+    assert lib.b200q_lora_add(16, 16, 16, 16, 16, None, None, 16, 2, 32, 64, 3, 4, 0, 8, 1 << 20, None) == -4
+    assert lib.b200q_lora_qmatvec(4, 16, 16, 16, 16, None, 16, 16, 16, None, None, 16, 2, 32, 64, 32, 3, 4, 0, 0, 24, 1 << 20, None) == -4
