@@ -73,6 +73,7 @@ int b200q_device_status(int reset, void* stream);
  *   "peer.spin_limit", "tp.spin_limit"   flag probes after which b200q_peer_allgather / the wait of an exchange fused
  *                        into a kernel gives up and records event 5 (default 2^22; tests shorten it)
  *   "lora.cluster"       CTAs per cluster of b200q_lora_add: 1, 2, 4, 8 or 16 (default: by rows)
+ *   "lora.fused"         b200q_lora_qmatvec of up to four rows in one launch: 1 wherever it can be, -1 nowhere (default: by rows, rank and K)
  *   "no_pdl"             1 = launch without programmatic dependent launch */
 int b200q_set_tuning(const char* key, int value);
 

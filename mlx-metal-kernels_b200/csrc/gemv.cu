@@ -360,6 +360,19 @@ int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scal
     return run_rows(bits, p, false, stream);
 }
 
+// Rows with adapters in one launch of the integer kernel; B200Q_ERR_UNSUPPORTED, with nothing launched, where that kernel is not the matvec's.
+int lora_rows_qmatvec(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y, int B,
+                      int64_t N, int64_t K, int group_size, int act_dtype, int scale_dtype, const LoraRows& lora, cudaStream_t stream) {
+    if (B > 4 || lora.R > kLoraRowsMaxRank || (reinterpret_cast<uintptr_t>(lora.a) & 15u) != 0) return B200Q_ERR_UNSUPPORTED;
+    GemvParams p = {};
+    p.x = x; p.w[0] = codes; p.s[0] = scales; p.z[0] = zeros; p.residual = residual; p.y = y; p.lora = lora;
+    p.B = B; p.N = (int)N; p.K = (int)K; p.G = group_size; p.Gn = (int)((K + group_size - 1) / group_size);
+    p.act_dtype = act_dtype; p.scale_dtype = scale_dtype;
+    p.row_bytes = bits == 4 ? (int)((K + 1) / 2) : (int)K;
+    if (tuning_get("gemv.i8") < 0 || prefer_ts(p) || !fast_path_ok(p)) return B200Q_ERR_UNSUPPORTED;
+    return bits == 4 ? gemv_i8_q4(p, false, stream) : gemv_i8_q8(p, false, stream);
+}
+
 int gate_up_impl(int bits, const void* x, const uint8_t* gate_codes, const uint8_t* up_codes, const void* gate_scales,
                  const void* up_scales, const void* gate_zeros, const void* up_zeros, void* gate_out, void* up_out,
                  void* act_out, const void* residual_in, const void* norm_weight, float eps, void* z_out,

@@ -74,6 +74,7 @@ struct I8Params {
     const __half* z[2];
     const void* residual;
     const float* add32;
+    LoraRows lora;
     void* y;
     void* gate_out;
     void* up_out;
@@ -86,7 +87,7 @@ struct I8Params {
     int batch;              // tiles whose sums fit into shared memory at once
     TpOut tp_out;
     TpIn tp_in;
-    uint32_t off_zero, off_xd, off_cst, off_res, off_part, off_meta, off_ring;
+    uint32_t off_zero, off_xd, off_cst, off_res, off_low, off_part, off_meta, off_ring;
     uint32_t xstride, cstride, meta_slot;
 };
 
@@ -261,14 +262,80 @@ template <int BITS, int LOGG> struct I8Shape {
 
 // What a kernel is compiled for: plain rows, packets of a tensor-parallel exchange, or fp32 rows added before the rounding (deciding on
 // the latter at run time made every other call 2 % longer: 4.62 -> 4.71 us for 4096 x 4096 q4).
-enum I8Mode : int { kI8Plain = 0, kI8Packets = 1, kI8Adds = 2 };
+// kI8Lora: adapters of the rows, whose first products every CTA forms for itself.
+enum I8Mode : int { kI8Plain = 0, kI8Packets = 1, kI8Adds = 2, kI8Lora = 3 };
+
+// A x of every row and rank, times the adapter's scaling, in fp32: a warp per value, low [B][R].  Bound by L2's latency: four rounds of four loads
+// for rows of 4096, while the CTA's weights are on their way (one row of rank 16 with a projection 4096 x 4096: 6.8 us, of which 4.4 without
+// adapters; eight loads of A at a time 7.5).
+__device__ __forceinline__ void i8_lora_low(const I8Params& p, float* low, int warp, int lane) {
+    const int R = p.lora.R;
+#pragma unroll 1
+    for (int at = warp; at < p.B * R; at += kI8Warps) {
+        const int b = at / R, r = at - b * R, id = p.lora.ids[b];
+        float s = 0.0f;
+        if (id >= 0 && id < p.lora.L && (p.lora.ranks == nullptr || r < p.lora.ranks[id])) {
+            const int64_t row = ((int64_t)id * R + r) * p.K, xrow = (int64_t)b * p.K;
+#pragma unroll 1
+            for (int k0 = lane * 8; k0 < p.K; k0 += 256 * 4) {
+                uint32_t a[4][4], x[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = k0 + 256 * j;
+                    a[j][0] = a[j][1] = a[j][2] = a[j][3] = x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0u;
+                    if (k < p.K) {
+                        i8_ldg(a[j], p.lora.a, row + k);
+                        i8_ldg(x[j], p.x, xrow + k);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float u[8], v[8];
+                    i8_words_to_f32(a[j], p.act_dtype, u);
+                    i8_words_to_f32(x[j], p.act_dtype, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s = fmaf(u[i], v[i], s);
+                }
+            }
+            s = i8_warp_sum(s);
+            if (p.lora.scaling != nullptr) s *= p.lora.scaling[id];
+        }
+        if (lane == 0) low[at] = s;
+    }
+}
+// What is added to column n of row b: residual + B low.
+__device__ __forceinline__ float i8_lora_value(const I8Params& p, const float* low, int b, int n) {
+    const int R = p.lora.R, id = p.lora.ids[b];
+    float s = 0.0f;
+    if (id >= 0 && id < p.lora.L) {
+        const int rank = p.lora.ranks == nullptr ? R : min(R, p.lora.ranks[id]);
+        const int64_t row = ((int64_t)id * p.N + n) * R;
+        low += b * R;
+        if (R % 8 == 0 && (reinterpret_cast<uintptr_t>(p.lora.b) & 15u) == 0) {
+#pragma unroll
+            for (int r0 = 0; r0 < kLoraRowsMaxRank; r0 += 8) {
+                if (r0 >= rank) break;
+                uint32_t w[4];
+                float v[8];
+                i8_ldg(w, p.lora.b, row + r0);
+                i8_words_to_f32(w, p.act_dtype, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (r0 + i < rank) s = fmaf(v[i], low[r0 + i], s);      // what lies behind the rank is not the adapter's
+            }
+        } else {
+            for (int r = 0; r < rank; ++r) s = fmaf(load_as_f32(p.lora.b, p.act_dtype, row + r), low[r], s);
+        }
+    }
+    return p.residual != nullptr ? load_as_f32(p.residual, p.act_dtype, (int64_t)b * p.N + n) + s : s;
+}
 
 // PB: bytes of a piece of scales, 16, 8 or 4, where rows of scales (and the units in them) start at multiples of it: pieces then lie in
 // shared memory as the affine step wants them, eight groups to a load.  0: rows that start anywhere; an aligned window is copied and read
 // one value at a time.  KS: CTAs per row, 1 or 2.  (PB at run time: 3 % slower.)
 template <int BITS, int LOGG, int NB, I8Mode MODE, int PB, int KS>
 __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_constant__ I8Params p) {
-    constexpr bool PACKETS = MODE == kI8Packets, ADDS = MODE == kI8Adds;
+    constexpr bool PACKETS = MODE == kI8Packets, LORA = MODE == kI8Lora, ADDS = MODE == kI8Adds || LORA;
     extern __shared__ __align__(128) uint8_t smem[];
     using S = I8Shape<BITS, LOGG>;
     constexpr int G = S::G, GB = S::GB, NM = S::NM, GU = S::GU, CP = S::CP, CH = S::CH, CG = S::CG, MB = S::MB, WIN = S::WIN;
@@ -372,7 +439,10 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
         __syncthreads();
     }
     const bool res_smem = (ADDS || p.residual != nullptr) && r_cnt * B <= kI8MaxRes;
-    if (res_smem)
+    if constexpr (LORA) {
+        if (rank == 0) i8_lora_low(p, reinterpret_cast<float*>(smem + p.off_low), warp, lane);
+        if (blockIdx.x == 0 && (int)threadIdx.x < B && p.lora.ids[threadIdx.x] >= p.lora.L) atomicMax(&g_device_status, (int)EV_LORA_ADAPTER);
+    } else if (res_smem)
         for (int i = threadIdx.x; i < r_cnt * B; i += kI8Threads) {
             const int b = i / r_cnt;
             if constexpr (ADDS) add[i] = p.add32[(size_t)b * p.N + r_lo + (i - b * r_cnt)];
@@ -472,6 +542,13 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
     }
     __syncthreads();
     if (KS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (LORA) {
+        if (rank == 0)
+            for (int i = threadIdx.x; i < r_cnt * B; i += kI8Threads) {
+                const int b = NB == 1 ? 0 : i / r_cnt;
+                add[i] = i8_lora_value(p, reinterpret_cast<const float*>(smem + p.off_low), b, r_lo + (i - b * r_cnt));
+            }
+    }
 
     // ---------------- per-lane constants of the consumer ----------------
     const int col_b = g >> 2;                          // batch row of this lane's B column inside a tile; one batch row: parity of the group
@@ -649,7 +726,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) qgemv_i8_kernel(const __grid_co
                 if (p.act_out != nullptr) reinterpret_cast<unsigned short*>(p.act_out)[o] = bits_of(v);
             } else {
                 if constexpr (ADDS) {
-                    v = (res_smem ? add[b * r_cnt + rb0 + rr] : p.add32[o]) + v;
+                    v = (LORA || res_smem ? add[b * r_cnt + rb0 + rr] : p.add32[o]) + v;
                 } else if (p.residual != nullptr) {
                     const uint16_t rb = res_smem ? resid[b * r_cnt + rb0 + rr] : reinterpret_cast<const uint16_t*>(p.residual)[o];
                     v = load_as_f32(&rb, p.act_dtype, 0) + v;
@@ -690,7 +767,7 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
         p.s[m] = (const __half*)q.s[m];
         p.z[m] = (const __half*)q.z[m];
     }
-    p.residual = q.residual; p.add32 = q.add32; p.y = q.y; p.gate_out = q.gate_out; p.up_out = q.up_out; p.act_out = q.act_out;
+    p.residual = q.residual; p.add32 = q.add32; p.lora = q.lora; p.y = q.y; p.gate_out = q.gate_out; p.up_out = q.up_out; p.act_out = q.act_out;
     p.eps = q.eps; p.B = q.B; p.N = q.N; p.K = q.K; p.Gn = q.Gn; p.act_dtype = q.act_dtype; p.norm_w_dtype = q.norm_w_dtype;
     p.row_bytes = q.row_bytes; p.tp_out = q.tp_out; p.tp_in = q.tp_in;
     p.units = (p.row_bytes + kI8UnitBytes - 1) / kI8UnitBytes;
@@ -703,7 +780,7 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
     while (pb > 0 && p.Gn * 2 % pb != 0) pb = pb == 16 ? P8 : pb == 8 ? P4 : 0;
     const int form = pb == 16 ? 3 : pb == 8 ? 2 : pb == 4 ? 1 : 0;
     p.meta_slot = 32u * (form ? S::MB : S::WIN * 16);
-    const bool packets = p.tp_in.world > 0 && p.tp_in.packets;
+    const bool packets = p.tp_in.world > 0 && p.tp_in.packets, lora = p.lora.a != nullptr;
     int ks = 1;
     const int tile_bytes = p.mats * p.units * 16 * NB * 4;
     int grid = 1;
@@ -720,7 +797,8 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
         p.off_zero = off;  off += S::XU + 128;
         p.off_xd = off;    off += i8_align((uint32_t)q.B * p.xstride, 128);
         p.off_cst = off;   off += (uint32_t)q.B * p.cstride;
-        p.off_res = off;   off += p.residual || p.add32 ? i8_align((uint32_t)std::min(r_max * q.B, kI8MaxRes) * (p.add32 ? 4 : 2), 128) : 0;
+        p.off_res = off;   off += p.residual || p.add32 || lora ? i8_align((uint32_t)std::min(r_max * q.B, kI8MaxRes) * (p.add32 || lora ? 4 : 2), 128) : 0;
+        p.off_low = off;   off += lora ? i8_align((uint32_t)q.B * p.lora.R * 4, 128) : 0;
         off = i8_align(off, 128);
         p.off_part = off;  off += i8_align((uint32_t)(p.batch * tile_bytes), 128);
         p.off_meta = off;  off += kI8Warps * 2 * p.meta_slot;
@@ -754,18 +832,19 @@ int launch_i8(const GemvParams& q, bool gate_up, cudaStream_t stream) {
         if (off2 <= (uint32_t)max_smem_optin() && (!fits || one - rounds() >= 2)) off = off2;
         else off = fit(1);
     }
-    if (off > (uint32_t)max_smem_optin()) return B200Q_ERR_UNSUPPORTED;
+    if (off > (uint32_t)max_smem_optin() || (lora && (p.rows_lo + 1) * p.B > kI8MaxRes)) return B200Q_ERR_UNSUPPORTED;
 
     using KernelFn = void (*)(I8Params);
 #define B200Q_I8_FORMS(MODE, KS)                                                                        \
     {qgemv_i8_kernel<BITS, LOGG, NB, MODE, 0, KS>, qgemv_i8_kernel<BITS, LOGG, NB, MODE, P4, KS>,       \
      qgemv_i8_kernel<BITS, LOGG, NB, MODE, P8, KS>, qgemv_i8_kernel<BITS, LOGG, NB, MODE, P16, KS>}
-    static const KernelFn kernels[6][4] = {B200Q_I8_FORMS(kI8Plain, 1), B200Q_I8_FORMS(kI8Packets, 1), B200Q_I8_FORMS(kI8Adds, 1),
-                                           B200Q_I8_FORMS(kI8Plain, 2), B200Q_I8_FORMS(kI8Packets, 2), B200Q_I8_FORMS(kI8Adds, 2)};
+    static const KernelFn kernels[8][4] = {
+        B200Q_I8_FORMS(kI8Plain, 1), B200Q_I8_FORMS(kI8Packets, 1), B200Q_I8_FORMS(kI8Adds, 1), B200Q_I8_FORMS(kI8Lora, 1),
+        B200Q_I8_FORMS(kI8Plain, 2), B200Q_I8_FORMS(kI8Packets, 2), B200Q_I8_FORMS(kI8Adds, 2), B200Q_I8_FORMS(kI8Lora, 2)};
 #undef B200Q_I8_FORMS
-    const int kind = (ks - 1) * 3 + (q.add32 != nullptr ? kI8Adds : packets ? kI8Packets : kI8Plain);
+    const int kind = (ks - 1) * 4 + (lora ? kI8Lora : q.add32 != nullptr ? kI8Adds : packets ? kI8Packets : kI8Plain);
     KernelFn kernel = kernels[kind][form];
-    static bool configured[24][64] = {};   // per instantiation and device; a race only repeats the call
+    static bool configured[32][64] = {};   // per instantiation and device; a race only repeats the call
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[kind * 4 + form][dev & 63]) {

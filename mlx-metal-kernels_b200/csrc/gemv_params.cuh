@@ -30,6 +30,17 @@ constexpr uint32_t kWaitLimit = 1u << 21;
 constexpr int kMaxStages = 8;
 constexpr int kMaxSlots = 16;
 
+// Adapters of a few rows, inside the integer matvec: y[b] += scaling[l] B[l] (A[l] x[b]), l = ids[b] (lora.cu has the formula and the operands)
+struct LoraRows {
+    const void* a;          // [L, R, K]; null: no adapters
+    const void* b;          // [L, N, R]
+    const float* scaling;   // [L] or null: 1
+    const int32_t* ranks;   // [L] or null: R
+    const int32_t* ids;     // [B]
+    int L, R;
+};
+constexpr int kLoraRowsMaxRank = 32;
+
 struct GemvParams {
     // activations
     const void* x;          // [B, K]
@@ -45,6 +56,7 @@ struct GemvParams {
     // outputs
     const void* residual;   // plain: out = cast(residual + cast(y)); may be null
     const float* add32;     // plain, instead of a residual: out = cast(add32 + y), [B, N]; may be null
+    LoraRows lora;          // plain: added before the rounding, beside the residual; integer kernel only
     void* y;
     void* gate_out;
     void* up_out;

@@ -14,10 +14,12 @@
 // and round, a lane with contiguous bytes of B again and 16 bytes of y, the next rounds' loads in flight during this one's products.  The
 // values between the factors enter the second product as two 16-bit terms, scaled by a power of two per row, which holds them to about 2^-21.
 //
+// Beside a projection of a few rows and small ranks none of this runs: the integer matvec takes the adapters along (lora_qmatvec_impl below).
+//
 // Bound by latency for a few rows (a chain of ids, first factor, two meetings, second factor: 5.9 us for one row of rank 16, 4096 x 4096, and
 // 13.5 for 32 rows of 24 adapters of rank 64, 6144 x 4096, 1.8 TB/s), by L2 and the products for prompts, whose groups of 16 rows read both factors
 // again (512 rows of rank 64, 14336 x 4096: 30 us).
-#include "common.cuh"
+#include "gemv_params.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -30,6 +32,8 @@ int qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void* scal
                  const void* residual, void* y, int B, int64_t N, int64_t K, int group_size, int act_dtype,
                  int scale_dtype, const void* residual_in, const void* norm_weight, int norm_w_dtype, float eps,
                  void* z_out, void* normed_out, cudaStream_t stream, const float* add32);
+int lora_rows_qmatvec(int bits, const void* x, const uint8_t* codes, const void* scales, const void* zeros, const void* residual, void* y, int B,
+                      int64_t N, int64_t K, int group_size, int act_dtype, int scale_dtype, const LoraRows& lora, cudaStream_t stream);
 
 namespace {
 
@@ -621,7 +625,11 @@ int lora_add_impl(const void* x, const void* y, void* out, const void* a, const 
     return lora_rows({x, y, out, a, b, scaling, ranks, ids, (float*)ws, rows, K, N, L, R, 0}, dtype, ws_bytes, stream);
 }
 
-// The adapters' rows in fp32, then the matvec that adds them before its one rounding.
+// A few rows of small ranks: one launch of the integer matvec, in which every CTA forms A x itself, as long as that takes its 16 warps eight rounds
+// of 1024 values or less.  Two launches -> one, us, rows / rank: 4096 x 4096 q4 1/16 10.9 -> 6.8, 1/32 11.0 -> 7.7, 2/16 12.6 -> 10.1, 4/8 14.0 -> 11.8;
+// 2048 x 2048 4/16 11.8 -> 10.7; 14336 x 4096 1/16 17.4 -> 11.5.  Beyond: 4096 x 4096 2/32 12.7 -> 13.4, 4/16 14.0 -> 16.2; 4096 x 14336 1/8 16.8 -> 17.5.
+constexpr int64_t kFusedRounds = 8;
+// More: the adapters' rows in fp32, then the matvec that adds them before its one rounding.
 static size_t low_rows_bytes(int64_t rows, int64_t N) { return (4 * (size_t)rows * (size_t)N + 255) / 256 * 256; }
 size_t lora_qmatvec_workspace_impl(int64_t rows, int64_t N, int R) {
     return rows <= 0 || N <= 0 || R <= 0 ? 0 : low_rows_bytes(rows, N) + lora_workspace_impl(rows, R);
@@ -635,6 +643,12 @@ int lora_qmatvec_impl(int bits, const void* x, const uint8_t* codes, const void*
         return B200Q_ERR_BAD_ARG;
     if (N > INT32_MAX || K > INT32_MAX) return B200Q_ERR_UNSUPPORTED;
     if (ws == nullptr || ((uintptr_t)ws & 15u) != 0 || ws_bytes < lora_qmatvec_workspace_impl(rows, N, R)) return B200Q_ERR_WORKSPACE;
+    const int fused = tuning_get("lora.fused");
+    if (fused >= 0 && rows <= 4 && (fused > 0 || (rows * (int64_t)R + 15) / 16 * ((K + 1023) / 1024) <= kFusedRounds)) {
+        const int rc = lora_rows_qmatvec(bits, x, codes, scales, zeros, residual, y, rows, N, K, group_size, act_dtype, scale_dtype,
+                                         {a, b, scaling, ranks, ids, L, R}, stream);
+        if (rc != B200Q_ERR_UNSUPPORTED) return rc;
+    }
     const size_t low = low_rows_bytes(rows, N);
     const int rc = lora_rows({x, residual, ws, a, b, scaling, ranks, ids, (float*)((uint8_t*)ws + low), rows, K, N, L, R, 1}, act_dtype, ws_bytes - low, stream);
     if (rc != B200Q_OK) return rc;

@@ -248,3 +248,88 @@ def test_thousands_of_rows_and_results_in_place(cuda, K, R):
     cabi.check(lib.b200q_lora_add(x.data_ptr(), y.data_ptr(), y.data_ptr(), ad.a.data_ptr(), ad.b.data_ptr(), ad.scaling.data_ptr(), None,
                                   ids.data_ptr(), rows, N, K, L, R, cabi.F16, ws.data_ptr(), ws.numel(), cabi.stream()), "b200q_lora_add")
     assert torch.equal(y, got)
+
+
+def exact_delta(x, ad, ids):
+    """scaling B (A x) in 64 bits, 0 without an adapter, and what fp32 sums may be off: K and then R products one after the other, 2^-24 of the
+    absolute sum each, the scaling, and the first sums' errors through B."""
+    rows, K = x.shape
+    L, R, _ = ad.a.shape
+    out = torch.zeros((rows, ad.b.shape[1]), dtype=torch.float64, device=x.device)
+    err = torch.zeros_like(out)
+    for t, l in enumerate(ids.tolist()):
+        if not 0 <= l < L:
+            continue
+        rank = R if ad.ranks is None else int(ad.ranks[l])
+        a, b, s = ad.a[l, :rank].double(), ad.b[l, :, :rank].double(), 1.0 if ad.scaling is None else float(ad.scaling[l])
+        low, low_abs = a @ x[t].double(), a.abs() @ x[t].double().abs()
+        out[t] = s * (b @ low)
+        err[t] = s * (b.abs() @ (K * 2.0 ** -24 * low_abs + (R + 4) * 2.0 ** -24 * low.abs()))
+    return out, err
+
+
+FEW = [  # rows, N, K, G, R
+    (1, 512, 1024, 64, 16), (1, 4096, 4096, 64, 16), (2, 1003, 2592, 32, 12), (3, 777, 512, 128, 5), (4, 640, 1056, 32, 8), (4, 148, 96, 32, 32),
+    (1, 100, 4096, 128, 32), (2, 5, 64, 32, 1), (1, 264, 14336, 64, 8), (4, 300, 8192, 64, 16),
+]
+
+
+@pytest.mark.parametrize("rows,N,K,G,R", FEW)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("fused", [0, 1, -1])
+def test_few_rows_beside_a_projection(cuda, bits, rows, N, K, G, R, dtype, fused):
+    """Off by the roundings of the sum and of the plain product it is compared with, and by what fp32 sums lose: in one launch and in two,
+    with residuals, rows without an adapter, an adapter that does not exist, and NaN behind the ranks."""
+    w, s, z = (t.to(cuda) for t in synth.quantized_weight(N, K, bits, G, seed=N))
+    x = synth.activations((rows, K), 2).to(dtype).to(cuda)
+    ranks = [R, max(R - 3, 0), R // 2]
+    ad = make(3, R, K, N, dtype, cuda, 3, ranks)
+    for l, rank in enumerate(ranks):
+        ad.a[l, rank:] = float("nan")
+        ad.b[l, :, rank:] = float("nan")
+    half = torch.finfo(dtype).eps / 2
+    base = mlp_ops.quantized_linear(x, w, s, z, bits=bits, group_size=G)
+    cabi.device_status()
+    cabi.set_tuning("lora.fused", fused)
+    try:
+        for first in (-1, 0, 1, 2):
+            ids = ((torch.arange(rows, dtype=torch.int32, device=cuda) + first + 1) % 4) - 1
+            delta, err = exact_delta(x, ad, ids)
+            for residual in (None, synth.activations((rows, N), 5).to(dtype).to(cuda)):
+                got = lora.lora_quantized_linear(x, w, s, z, ad, ids, bits=bits, group_size=G, residual=residual)
+                assert torch.equal(got, lora.lora_quantized_linear(x, w, s, z, ad, ids, bits=bits, group_size=G, residual=residual))
+                rest = 0.0 if residual is None else residual.double()
+                want = base.double() + delta + rest
+                size = base.double().abs() + delta.abs() + (0.0 if residual is None else rest.abs())
+                bound = half * (1 + 4 * half) * (want.abs() + base.double().abs()) + (1 + half) * err + 2.0 ** -22 * size + 2.0 ** -24
+                assert bool(((got.double() - want).abs() <= bound).all())
+                if residual is None:
+                    assert torch.equal(got[ids < 0], base[ids < 0])
+        assert cabi.device_status() == 0
+        missing = torch.full((rows,), 3, dtype=torch.int32, device=cuda)
+        assert torch.equal(lora.lora_quantized_linear(x, w, s, z, ad, missing, bits=bits, group_size=G), base)
+        assert cabi.device_status() == 10
+    finally:
+        cabi.set_tuning("lora.fused", 0)
+
+
+def test_few_rows_captured(cuda):
+    """One launch, captured: a replay reads new rows, ids, ranks and scalings."""
+    K, N = 2048, 768
+    w, s, z = (t.to(cuda) for t in synth.quantized_weight(N, K, 4, 64, seed=1))
+    ad = make(4, 8, K, N, torch.bfloat16, cuda, 12, [8, 3, 0, 5])
+    x = synth.activations((2, K), 3).to(torch.bfloat16).to(cuda)
+    ids = torch.tensor([1, -1], dtype=torch.int32, device=cuda)
+    call = lambda: lora.lora_quantized_linear(x, w, s, z, ad, ids, group_size=64)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    x.copy_(synth.activations((2, K), 4))
+    ids.copy_(torch.tensor([3, 0]))
+    ad.ranks.copy_(torch.tensor([2, 3, 0, 8]))
+    ad.scaling.mul_(2.0)
+    graph.replay()
+    assert torch.equal(out, call())
