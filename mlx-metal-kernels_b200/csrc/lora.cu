@@ -583,8 +583,9 @@ template <typename T> int cluster_form(const LoraParams& p, cudaStream_t stream)
     void (*kernel)(const LoraParams, int, int, int) =
         sliced ? (narrow ? lora_cluster_kernel<T, 2, 8, true> : wide ? lora_cluster_kernel<T, 8, 8, true> : lora_cluster_kernel<T, 4, 8, true>)
                : (narrow ? lora_cluster_kernel<T, 2, 8, false> : wide ? lora_cluster_kernel<T, 8, 8, false> : lora_cluster_kernel<T, 4, 8, false>);
-    if (smem > 40 * 1024 &&      // with the static part beyond what needs no asking
-         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    if (smem > 40 * 1024 &&      // with the static part beyond what needs no asking (one value for all calls: two threads may launch the same kernel)
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lora_smem(kMaxRank, warps, ring_depth(8)).bytes) != cudaSuccess)
+        return B200Q_ERR_LAUNCH;
     if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return B200Q_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * ctas));

@@ -780,7 +780,8 @@ int ring(const RopeParams& params, bool half_layout, int log_lanes, cudaStream_t
     const bool norm = p.weight[0] != nullptr || p.weight[1] != nullptr;
     void (*kernel)(const RingParams, int) = half_layout ? (run == 1 ? (norm ? rope_ring_kernel<T, true, CACHE, 1, true> : rope_ring_kernel<T, true, CACHE, 1, false>) : rope_ring_kernel<T, true, CACHE, 2, true>)
                                                         : (run == 1 ? (norm ? rope_ring_kernel<T, false, CACHE, 1, true> : rope_ring_kernel<T, false, CACHE, 1, false>) : rope_ring_kernel<T, false, CACHE, 2, true>);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return B200Q_ERR_LAUNCH;
+    // (one value for all calls: two threads may launch the same kernel with different sizes)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes) != cudaSuccess) return B200Q_ERR_LAUNCH;
     return launch(kernel, std::min<int64_t>(p.T, (int64_t)sm_count() * 2), rp.consumers + 32, smem, stream, rp, log_lanes);
 }
 

@@ -1,6 +1,7 @@
 """The operators as a serving loop uses them together: projections with adapters, head norms with rotation and append, decode attention,
 and pages reserved, forked, released and compacted under it."""
 import importlib
+import threading
 
 import pytest
 import torch
@@ -129,3 +130,40 @@ def test_a_serving_loop(cuda, bits):
     want = torch.einsum("hn,nhd->hd", scores.softmax(-1), v.repeat_interleave(group, 1))
     # fp16 probabilities and output of the attention kernel: as its own parity tests allow
     assert float((captured[i][b, 0].double() - want).abs().max()) <= 2e-3 * float(want.abs().max().clamp_min(1.0))
+
+
+def test_two_host_threads(cuda):
+    """The same kernels launched by two threads with other sizes of shared memory, each on a stream of its own."""
+    T = 8 * torch.cuda.get_device_properties(cuda).multi_processor_count + 5
+    jobs = []
+    for heads, R in ((4, 64), (24, 256)):
+        g = gen(heads)
+        x = torch.randn((T, heads, D), generator=g).half().to(cuda)
+        cos, sin = rope_ops.rotary_tables(rope_ops.RotaryConfig(head_dim=D), 64, cuda)
+        pos = (torch.arange(T) % 64).to(cuda)                              # int64: through the Python body, which lets go of the interpreter
+        a, b = torch.randn((2, R, K), generator=g).half().to(cuda), (torch.randn((2, 640, R), generator=g) * 0.1).half().to(cuda)
+        rows, y = torch.randn((20, K), generator=g).half().to(cuda), torch.randn((20, 640), generator=g).half().to(cuda)
+        ids = (torch.arange(20, dtype=torch.int32) % 3 - 1).to(cuda)
+        jobs.append(lambda x=x, cos=cos, sin=sin, pos=pos, a=a, b=b, rows=rows, y=y, ids=ids:
+                    (rope_ops.apply_rope(x, None, cos, sin, pos)[0], lora.lora_add(y, rows, lora.LoraAdapters(a, b), ids)))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(job, expected):
+        try:
+            with torch.cuda.device(cuda), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(150):
+                    got = job()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, expected)):
+                    wrong.append("results")
+        except Exception as e:                                             # noqa: BLE001 - shown by the assertion below
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=run, args=pair) for pair in zip(jobs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [] and cabi.device_status() == 0
